@@ -20,6 +20,7 @@ FLAG_HALF_STATE = 2
 FLAG_TAIL_KEEP = 4
 FLAG_SPLIT_CHANNELS = 8
 FLAG_NO_SPLIT_CHANNELS = 16
+FLAG_TAIL_START = 32
 FLAG_SELFTEST_MUTE_K = 0x80000000
 ABI_VERSION = 2
 
@@ -63,16 +64,30 @@ SIGNATURES = {
     "adkv_decode_attn": [c_void_p] * 10 + [c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                          c_float, c_float, c_float, c_uint, c_void_p],
     "adkv_decode_attn_varlen": [c_void_p] * 11 + [c_int] * 6 + [c_float, c_float, c_float, c_uint, c_void_p],
+    "adkv_decode_attn_prefix_scratch_bytes": [c_int] * 5,
+    "adkv_decode_attn_prefix": [c_void_p] * 11 + [c_int, c_void_p, c_void_p, c_longlong] + [c_int] * 6 + [c_float] * 3 + [c_uint, c_void_p],
+    "adkv_norm_rope_qkv": [c_void_p, c_longlong, c_longlong, c_int] + [c_void_p] * 3 + [c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                           c_longlong, c_int, c_int, c_void_p] + [c_int] * 8 + [c_void_p],
+    "adkv_process_logits": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_longlong, c_int, c_void_p,
+                            c_void_p, c_float, c_void_p, c_float, c_void_p, c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int,
+                            c_void_p],
     "adkv_device_status": [c_void_p, c_void_p],
     "adkv_selftest_wait_timeout": [c_int, c_void_p],
 }
-_RESTYPE = {"adkv_strerror": ctypes.c_char_p, "adkv_decode_attn_ckpt_scratch_bytes": c_longlong}
+_RESTYPE = {"adkv_strerror": ctypes.c_char_p, "adkv_decode_attn_ckpt_scratch_bytes": c_longlong,
+            "adkv_decode_attn_prefix_scratch_bytes": c_longlong}
 
 
 class Params(ctypes.Structure):
     """``adkv_params``: five fp16 ``[Hkv, D]`` device pointers."""
     _fields_ = [("zp_init", c_void_p), ("scale_init", c_void_p), ("alpha", c_void_p),
                 ("beta", c_void_p), ("target", c_void_p)]
+
+
+class Prefix(ctypes.Structure):
+    """``adkv_prefix``: the packed tokens that several sequences share."""
+    _fields_ = [("k_cache", c_void_p), ("v_cache", c_void_p), ("k_tail", c_void_p), ("v_tail", c_void_p), ("k_ckpt", c_void_p),
+                ("v_ckpt", c_void_p), ("tokens", c_int), ("n_super_cap", c_int), ("interval", c_int), ("n_ckpt_cap", c_int)]
 
 
 class LayerKV(ctypes.Structure):

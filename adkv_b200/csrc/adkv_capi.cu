@@ -11,6 +11,8 @@ ADKV_HIDDEN int adkv_tu_status_half(int *out);
 ADKV_HIDDEN int adkv_tu_status_narrow(int *out);
 ADKV_HIDDEN int adkv_tu_status_segments(int *out);
 ADKV_HIDDEN int adkv_tu_status_tensor(int *out);
+ADKV_HIDDEN int adkv_tu_status_prefix(int *out);
+ADKV_HIDDEN int adkv_tu_status_step(int *out);
 
 namespace adkv {
 
@@ -50,6 +52,7 @@ const char *adkv_strerror(int code)
     case ADKV_E_FLAGS:
         return "adkv: flag or optional argument not available in this combination (tail states need both tensors and "
                "the fp32 arithmetic)";
+    case ADKV_E_TYPE: return "adkv: element types not available in this combination";
     case ADKV_E_STATIC_MAX:
         return "adkv: problem needs more than the 16 MiB of built-in scratch (ADKV_STATIC_SCRATCH_BYTES); use "
                "adkv_decode_attn_ckpt with caller-owned scratch, or a larger checkpoint interval";
@@ -62,7 +65,7 @@ int adkv_device_status(int *status, void *stream)
     if (!status) return ADKV_E_NULL;
     const cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return int(e);
-    int a = 0, b = 0, c = 0, d = 0, w = 0, t = 0, hf = 0, nr = 0, sg = 0, tn = 0;
+    int a = 0, b = 0, c = 0, d = 0, w = 0, t = 0, hf = 0, nr = 0, sg = 0, tn = 0, pf = 0, st = 0;
     if (int rc = adkv_tu_status_fused(&a)) return rc;
     if (int rc = adkv_tu_status_unfused(&b)) return rc;
     if (int rc = adkv_tu_status_encode(&c)) return rc;
@@ -73,8 +76,12 @@ int adkv_device_status(int *status, void *stream)
     if (int rc = adkv_tu_status_narrow(&nr)) return rc;
     if (int rc = adkv_tu_status_segments(&sg)) return rc;
     if (int rc = adkv_tu_status_tensor(&tn)) return rc;
+    if (int rc = adkv_tu_status_prefix(&pf)) return rc;
+    if (int rc = adkv_tu_status_step(&st)) return rc;
+    if (st) nr = st;
     if (sg) nr = sg;
     if (tn) nr = tn;
+    if (pf) nr = pf;
     *status = a ? a : (b ? b : (c ? c : (d ? d : (w ? w : (hf ? hf : (nr ? nr : t))))));
     return 0;
 }

@@ -159,6 +159,7 @@ struct CkptSpec {
     int interval;     // tokens between checkpoints (multiple of 32), 0 = none
     int n_ckpt_cap;
     int D;            // head dim (128, 256 or 512); a CTA handles one 128-channel slice of one stream
+    bool from_tail = false;   // prefill: start from the tails (always so behind the first token)
 };
 constexpr int kEncMaxTensors = 16;   // tensors per launch: K and V of up to 8 layers (the struct is a kernel parameter)
 struct EncBatch {
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kD / CPT) encode_kernel(EncBatch batch, CkptSp
         Io::get(*reinterpret_cast<const Half *>(p.alpha + po), al);
         Io::get(*reinterpret_cast<const Half *>(p.beta + po), beta);
         Io::get(*reinterpret_cast<const Half *>(p.target + po), target);
-        if (t_start > 0) {
+        if (cs.from_tail) {
             Io::get(*reinterpret_cast<const Float *>(tail + size_t(bh) * 2 * D + c0), zp);
             Io::get(*reinterpret_cast<const Float *>(tail + size_t(bh) * 2 * D + D + c0), sc);
         } else {
@@ -517,6 +518,7 @@ static int launch_encode(const EncBatch &b, int n, int B, int H, int T, int D, i
 {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cs.D = D;
+    cs.from_tail = cs.from_tail || t_start > 0;
     const int n_slices = B * H * (D / kD);
     const long long grid = (long long)n_slices * n;
     // One channel per thread while that leaves a warp scheduler at most three warps: a warp then has its scheduler (nearly)
@@ -610,6 +612,22 @@ int adkv_encode_kv_flags(void *k_cache, const void *k, const adkv_params *kp, vo
 {
     const bool pair = v_cache != nullptr;
     if (interval < 0 || (interval > 0 && !pair)) return ADKV_E_SHAPE;   // checkpoints are kept for K and V together
+    if (flags & ADKV_FLAG_TAIL_START) {
+        if (flags & ADKV_FLAG_HALF_STATE) return ADKV_E_FLAGS;
+        if (t_start < 0) return ADKV_E_SHAPE;
+        if (int rc = encode_check(k_cache, k, kp, k_tail, T, 1)) return rc;
+        if (pair)
+            if (int rc = encode_check(v_cache, v, vp, v_tail, T, 1)) return rc;
+        if (int rc = check_common(B, H, H, T, D, n_super_cap, bits, t_start + T)) return rc;
+        if (interval > 0)
+            if (int rc = ckpt_check(k_ckpt, v_ckpt, interval, n_ckpt_cap, t_start + T)) return rc;
+        if (B * H == 0 || T == 0) return 0;
+        EncBatch b{};
+        b.t[0] = enc_tensor(k_cache, k, kp, k_tail, interval ? k_ckpt : nullptr);
+        if (pair) b.t[1] = enc_tensor(v_cache, v, vp, v_tail, interval ? v_ckpt : nullptr);
+        return launch_encode(b, pair ? 2 : 1, B, H, T, D, n_super_cap, bits, t_start, scale_min, scale_max, stream,
+                             CkptSpec{interval, n_ckpt_cap, D, true});
+    }
     if (!(flags & ADKV_FLAG_HALF_STATE)) {
         if (interval > 0)
             return adkv_encode_kv_ckpt(k_cache, k, kp, k_tail, k_ckpt, v_cache, v, vp, v_tail, v_ckpt, interval, n_ckpt_cap,

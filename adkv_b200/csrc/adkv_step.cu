@@ -1,0 +1,486 @@
+// Part of libadkv_b200.so (sm_100a).  See include/adkv_b200.h for the contract of every entry point.
+//
+// What a decode or prefill step does around the attention kernels: the rotation (and normalisation per head) of queries and keys
+// between the projection and the cache, and the penalties, biases and masks on the logits with the choice of the next token.
+#include "adkv_host.h"
+
+#include <cuda_bf16.h>
+
+namespace adkv {
+
+constexpr int kStatPosition = 8;   // a position held on the device lies outside the rotation tables
+
+// Four consecutive elements of a row, as floats.
+__device__ __forceinline__ void load4(float (&v)[4], const __half *p) { load_half4(v, p); }
+__device__ __forceinline__ void load4(float (&v)[4], const __nv_bfloat16 *p)
+{
+    const uint2 a = *reinterpret_cast<const uint2 *>(p);
+    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+    v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load4(float (&v)[4], const float *p)
+{
+    const float4 a = *reinterpret_cast<const float4 *>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void store4(__half *p, const float (&v)[4]) { store_half4(p, v); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&v)[4])
+{
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+
+// =========================================================================================
+// Rotation of queries and keys, with the root-mean-square norm of each head before it:
+//   y = x / sqrt(mean(x^2) + eps) * w          (w given)
+//   (a, b) -> (a cos - b sin, b cos + a sin)   for the rot / 2 pairs of channels: (i, i + rot / 2), or (2i, 2i + 1) interleaved
+// in fp32, one rounding at the end; products and sums of the rotation are rounded one by one, as the torch expression in e2e_llama
+// does.  Values pass through, so that all of [B, T, (Hq + 2 Hkv) D] leaves in the [B, H, T, D] layout that the caches take.
+//
+// Bound by memory: every element is read and written once, the tables are 1 % of it.  A lane holds eight channels of a head, four
+// pairs, so that both halves of a pair are its own and nothing but the sum of squares crosses lanes; D / 8 lanes share a head, and a
+// thread takes the same channels of up to kRopeRows heads of one token, so cosines and sines are loaded once for them and their
+// loads are in flight together.
+struct RopeArgs {
+    const void *qkv;
+    long long stride_b, stride_t;      // elements
+    void *q, *k, *v;
+    const void *q_weight, *k_weight;   // [D] in the input's type, or nullptr
+    const float *cos, *sin;            // [table_rows, >= rot / 2]
+    const int *positions;              // [B] (per_token false: of the first token) or [B, T], or nullptr
+    long long table_stride;
+    int table_rows, rot, per_token, start, T, Hq, Hkv, interleaved;
+    float eps;
+};
+constexpr int kRopeThreads = 256, kRopeRows = 4;
+
+template <int D, class In, class Out>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ RopeArgs a)
+{
+    constexpr int UNITS = D == 512 ? 2 : 1, LANES = D / 8 / UNITS;   // lanes of a head, and groups of eight channels of a lane
+    constexpr int HEADS = kRopeThreads / LANES;                      // heads that the CTA takes side by side
+    const int token = blockIdx.x, b = token / a.T, t = token % a.T;
+    const int lane = threadIdx.x % LANES, H = a.Hq + 2 * a.Hkv, half = a.rot / 2;
+    int pos = a.start + t;
+    if (a.positions) pos = a.per_token ? a.positions[token] : a.positions[b] + t;
+    const bool inside = pos >= 0 && pos < a.table_rows;
+    if (!inside && threadIdx.x == 0 && blockIdx.y == 0) atomicExch(&g_status, kStatPosition);
+
+    // first channels of the lane's two groups of four: pairs (first, second), or channels that are left as they are
+    int at0[UNITS], at1[UNITS];
+    float c[UNITS][4], s[UNITS][4];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int pair = 4 * (lane + LANES * u);
+        const bool turned = pair < half, split = turned && !a.interleaved;
+        at0[u] = split ? pair : 2 * pair;
+        at1[u] = split ? pair + half : 2 * pair + 4;
+        if (turned) {
+            const float bad = __int_as_float(0x7fc00000);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[u][i] = inside ? a.cos[(long long)pos * a.table_stride + pair + i] : bad;
+                s[u][i] = inside ? a.sin[(long long)pos * a.table_stride + pair + i] : bad;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { c[u][i] = inside ? 1.f : __int_as_float(0x7fc00000); s[u][i] = 0.f; }
+        }
+    }
+    const In *src = static_cast<const In *>(a.qkv) + b * a.stride_b + t * a.stride_t;
+    const int h0 = blockIdx.y * HEADS * kRopeRows + threadIdx.x / LANES;
+    float x[kRopeRows][UNITS][2][4];
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r)
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int h = h0 + HEADS * r;
+            if (h < H) {
+                load4(x[r][u][0], src + h * D + at0[u]);
+                load4(x[r][u][1], src + h * D + at1[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[r][u][0][i] = x[r][u][1][i] = 0.f;
+            }
+        }
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r) {
+        const int h = h0 + HEADS * r;
+        const bool is_v = h >= a.Hq + a.Hkv;
+        const In *weight = static_cast<const In *>(h < a.Hq ? a.q_weight : a.k_weight);
+        const bool norm = !is_v && weight;
+        if (a.q_weight || a.k_weight) {   // the same for all: the lanes of other heads take part in the sum
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum = fmaf(x[r][u][i / 4][i % 4], x[r][u][i / 4][i % 4], sum);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+            if (norm) {
+                const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    float w0[4], w1[4];
+                    load4(w0, weight + at0[u]);
+                    load4(w1, weight + at1[u]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[r][u][0][i] *= inv * w0[i];
+                        x[r][u][1][i] *= inv * w1[i];
+                    }
+                }
+            }
+        }
+        if (h >= H) continue;
+        Out *dst = is_v ? static_cast<Out *>(a.v) + (((long long)b * a.Hkv + h - a.Hq - a.Hkv) * a.T + t) * D
+                        : h < a.Hq ? static_cast<Out *>(a.q) + (((long long)b * a.Hq + h) * a.T + t) * D
+                                   : static_cast<Out *>(a.k) + (((long long)b * a.Hkv + h - a.Hq) * a.T + t) * D;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            float(&p)[4] = x[r][u][0], (&n)[4] = x[r][u][1];
+            const auto turn = [](float &first, float &second, float co, float si) {
+                const float was = first;
+                first = __fsub_rn(__fmul_rn(was, co), __fmul_rn(second, si));
+                second = __fadd_rn(__fmul_rn(second, co), __fmul_rn(was, si));
+            };
+            if (!is_v) {
+                if (a.interleaved) {
+                    turn(p[0], p[1], c[u][0], s[u][0]); turn(p[2], p[3], c[u][1], s[u][1]);
+                    turn(n[0], n[1], c[u][2], s[u][2]); turn(n[2], n[3], c[u][3], s[u][3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) turn(p[i], n[i], c[u][i], s[u][i]);
+                }
+            }
+            store4(dst + at0[u], p);
+            store4(dst + at1[u], n);
+        }
+    }
+}
+
+// =========================================================================================
+// Logits of a row, in fp32 and rounded once at the end:
+//   n = how often the token is in the row's history;  if n > 0:  x = x > 0 ? x / repetition : x * repetition,
+//   x = x - (frequency * n + presence);   then x + bias, and -inf where the mask's bit is not set.
+// The token is the lowest index of the largest result (a NaN counts as larger than anything), -1 where all are -inf.
+//
+// Bound by memory for a batch, by latency for one row.  A cluster of up to eight CTAs shares a row; each counts the history's tokens
+// that fall into its part in shared memory (integer additions, so the order does not matter) and then passes over its part once, 16
+// aligned bytes a load whatever the row's alignment; the CTAs' largest values meet in the shared memory of the first, so nothing
+// has to be cleared, kept or launched besides.
+struct LogitArgs {
+    const void *x;
+    void *out;
+    int *tokens;                                             // [B] or nullptr
+    const int *history, *history_lens;                       // [B, history_cap], [B] (nullptr: all of it)
+    const float *repetition, *presence, *frequency;          // [B], or nullptr: the number beside it
+    float repetition1, presence1, frequency1;
+    const float *bias;                                       // [V] (stride 0) or [B, V], or nullptr
+    const uint32_t *mask;                                    // [B, >= (V + 31) / 32], or nullptr
+    long long stride_x, stride_out, stride_history, stride_bias, stride_mask;
+    int V, history_cap;
+    int part;                                                // packs of a CTA, see below
+};
+constexpr int kLogitThreads = 512, kLogitChunk = 14336, kLogitCluster = 8;   // tokens counted at a time: 56 KB
+
+template <class T>
+struct LogitIo;
+template <>
+struct LogitIo<float> {
+    static constexpr int N = 4;
+    __device__ static float load(const float *p) { return *p; }
+    __device__ static void unpack(const uint4 &v, float (&x)[4])
+    {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+    __device__ static uint4 pack(const float (&x)[4])
+    {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    __device__ static float round(float v) { return v; }
+    __device__ static void store(float *p, float v) { *p = v; }
+};
+template <>
+struct LogitIo<__half> {
+    static constexpr int N = 8;
+    __device__ static float load(const __half *p) { return __half2float(*p); }
+    __device__ static void unpack(const uint4 &v, float (&x)[8])
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    }
+    __device__ static uint4 pack(const float (&x)[8])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float round(float v) { return __half2float(__float2half_rn(v)); }
+    __device__ static void store(__half *p, float v) { *p = __float2half_rn(v); }
+};
+template <>
+struct LogitIo<__nv_bfloat16> {
+    static constexpr int N = 8;
+    __device__ static float load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+    __device__ static void unpack(const uint4 &v, float (&x)[8])
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    __device__ static uint4 pack(const float (&x)[8])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+    __device__ static void store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+};
+
+// Value and index as one number whose order is that of the choice: larger values first (NaN above all, -0 as +0), then lower indexes.
+__device__ __forceinline__ unsigned long long rank_of(float v, int index)
+{
+    const uint32_t u = __float_as_uint(v + 0.f);
+    const uint32_t key = v != v ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
+    return (unsigned long long)key << 32 | uint32_t(~index);
+}
+constexpr uint32_t kRankMinusInf = 0x007fffffu;   // key of -inf
+
+// A pack: the elements of 16 aligned bytes of the row.  A row that starts `skew` elements behind such a boundary has elements
+// p * N - skew ... of pack p; of the first and the last one some lie outside.
+template <class T>
+__global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(const __grid_constant__ LogitArgs a)
+{
+    using Io = LogitIo<T>;
+    constexpr int N = Io::N;
+    extern __shared__ __align__(16) uint32_t counts[];
+    __shared__ unsigned long long best[kLogitThreads / 32], gathered[kLogitCluster];
+    uint32_t rank, ranks;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // that all CTAs of the cluster run is waited for below
+
+    const int b = blockIdx.y;
+    const T *x = static_cast<const T *>(a.x) + b * a.stride_x;
+    T *out = static_cast<T *>(a.out) + b * a.stride_out;
+    const float *bias = a.bias ? a.bias + b * a.stride_bias : nullptr;
+    const uint32_t *mask = a.mask ? a.mask + b * a.stride_mask : nullptr;
+    const int n_words = (a.V + 31) / 32;
+    const int skew = int(reinterpret_cast<uintptr_t>(x) / sizeof(T) % N);
+    const bool same = int(reinterpret_cast<uintptr_t>(out) / sizeof(T) % N) == skew;   // else the results are stored one by one
+    const int packs = (a.V + skew + N - 1) / N, p_end = min(packs, int(rank + 1) * a.part);
+    const float rep = a.repetition ? a.repetition[b] : a.repetition1, pres = a.presence ? a.presence[b] : a.presence1,
+                freq = a.frequency ? a.frequency[b] : a.frequency1;
+    const int *history = a.history ? a.history + b * a.stride_history : nullptr;
+    const int n_history = !history ? 0 : a.history_lens ? min(max(a.history_lens[b], 0), a.history_cap) : a.history_cap;
+
+    unsigned long long top = 0;
+    constexpr int kPacks = kLogitChunk / N;
+    for (int p0 = int(rank) * a.part; p0 < p_end; p0 += kPacks) {
+        const int p1 = min(p_end, p0 + kPacks), v0 = p0 * N - skew;
+        if (n_history) {
+            for (int i = threadIdx.x; i < (p1 - p0) * N / 4; i += kLogitThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            const uint32_t n = uint32_t((p1 - p0) * N);
+            for (int i = threadIdx.x; i < n_history; i += kLogitThreads) {
+                const int id = history[i];
+                if (id >= 0 && id < a.V && uint32_t(id - v0) < n) atomicAdd(&counts[id - v0], 1u);
+            }
+            __syncthreads();
+        }
+        for (int p = p0 + threadIdx.x; p < p1; p += kLogitThreads) {
+            const int v = p * N - skew;                    // index of the pack's first element
+            const bool whole = v >= 0 && v + N <= a.V;
+            float y[N];
+            if (whole) {
+                Io::unpack(*reinterpret_cast<const uint4 *>(x + v), y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = v + i >= 0 && v + i < a.V ? Io::load(x + v + i) : 0.f;
+            }
+            if (n_history) {
+                uint32_t n[N], any = 0;
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const uint4 c = *reinterpret_cast<const uint4 *>(counts + (p - p0) * N + i);
+                    n[i] = c.x; n[i + 1] = c.y; n[i + 2] = c.z; n[i + 3] = c.w;
+                    any |= c.x | c.y | c.z | c.w;
+                }
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (n[i]) {
+                            const float z = y[i] > 0.f ? __fdiv_rn(y[i], rep) : __fmul_rn(y[i], rep);
+                            y[i] = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(n[i])), pres));
+                        }
+                }
+            }
+            if (bias) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (whole || (v + i >= 0 && v + i < a.V)) y[i] = __fadd_rn(y[i], bias[v + i]);
+            }
+            if (mask) {
+                const int at = max(v, 0);
+                const uint32_t w0 = mask[at >> 5], w1 = mask[min((at >> 5) + 1, n_words - 1)];
+                const uint32_t bits = __funnelshift_r(w0, w1, at & 31) << (at - v);
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (!(bits >> i & 1)) y[i] = -INFINITY;
+            }
+            if (whole && same) {
+                *reinterpret_cast<uint4 *>(out + v) = Io::pack(y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (v + i >= 0 && v + i < a.V) Io::store(out + v + i, y[i]);
+            }
+            if (a.tokens) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (whole || (v + i >= 0 && v + i < a.V)) top = max(top, rank_of(Io::round(y[i]), v + i));
+            }
+        }
+        __syncthreads();   // the counts are read
+    }
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (!a.tokens) return;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+    if (threadIdx.x % 32 == 0) best[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kLogitThreads / 32; ++i) top = max(top, best[i]);
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(smem_u32(&gathered[rank])));
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(there), "l"(top) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && threadIdx.x == 0) {
+        for (uint32_t i = 0; i < ranks; ++i) top = max(top, gathered[i]);
+        a.tokens[b] = uint32_t(top >> 32) <= kRankMinusInf ? -1 : int(~uint32_t(top));
+    }
+}
+
+}  // namespace adkv
+
+using namespace adkv;
+
+ADKV_DEFINE_TU_STATUS(adkv_tu_status_step)
+
+template <int D>
+static int launch_rope(const RopeArgs &a, int B, int in_type, int out_type, cudaStream_t s)
+{
+    constexpr int heads = kRopeThreads / (D / 8 / (D == 512 ? 2 : 1)) * kRopeRows;
+    const dim3 grid(unsigned(B) * unsigned(a.T), (a.Hq + 2 * a.Hkv + heads - 1) / heads);
+    switch (in_type * 4 + out_type) {
+    case ADKV_T_F16 * 4 + ADKV_T_F16: norm_rope_kernel<D, __half, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
+    case ADKV_T_BF16 * 4 + ADKV_T_F16: norm_rope_kernel<D, __nv_bfloat16, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
+    case ADKV_T_BF16 * 4 + ADKV_T_BF16: norm_rope_kernel<D, __nv_bfloat16, __nv_bfloat16><<<grid, kRopeThreads, 0, s>>>(a); break;
+    case ADKV_T_F32 * 4 + ADKV_T_F16: norm_rope_kernel<D, float, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
+    case ADKV_T_F32 * 4 + ADKV_T_F32: norm_rope_kernel<D, float, float><<<grid, kRopeThreads, 0, s>>>(a); break;
+    default: return ADKV_E_TYPE;
+    }
+    return launch_status();
+}
+
+static bool aligned_to(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <class T>
+static int launch_logits(LogitArgs a, int B, cudaStream_t s)
+{
+    constexpr int N = LogitIo<T>::N;
+    // CTAs of a row: more until the launch fills the chip twice over or a CTA has fewer than 2048 elements
+    int cluster = 1;
+    while (cluster < kLogitCluster && (long long)B * cluster < 2 * kSMs && a.V / (2 * cluster) >= 2048) cluster *= 2;
+    while (cluster < kLogitCluster && a.history && a.V / cluster > kLogitChunk) cluster *= 2;   // each counts its part at once
+    const int packs = (a.V + 2 * N - 2) / N;   // of the worst alignment
+    a.part = (packs + cluster - 1) / cluster;
+    const int bytes = a.history ? min(a.part * N, kLogitChunk) * 4 : 0;
+    const auto kernel = process_logits_kernel<T>;
+    if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitChunk * 4) != cudaSuccess) return launch_status();
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(cluster, B);
+    cfg.blockDim = dim3(kLogitThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return launch_status();
+    return launch_status();
+}
+
+extern "C" {
+
+int adkv_norm_rope_qkv(const void *qkv, long long stride_b, long long stride_t, int in_type, void *q, void *k, void *v, int out_type,
+                       const void *q_weight, const void *k_weight, float eps, const void *cos, const void *sin, long long table_stride,
+                       int table_rows, int rot, const void *positions, int positions_per_token, int start, int B, int T, int Hq, int Hkv,
+                       int D, int interleaved, void *stream)
+{
+    if (!qkv || !q || !k || !v || !cos || !sin) return ADKV_E_NULL;
+    if (D != 64 && D != 128 && D != 256 && D != 512) return ADKV_E_HEAD_DIM;
+    if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || rot <= 0 || rot > D || rot % 8 || table_rows < 0 || start < 0 || stride_b % 4 || stride_t % 4 ||
+        (long long)B * T > 0x7fffffffll)
+        return ADKV_E_SHAPE;
+    if (in_type < ADKV_T_F16 || in_type > ADKV_T_F32 || (out_type != in_type && out_type != ADKV_T_F16)) return ADKV_E_TYPE;
+    const unsigned in4 = in_type == ADKV_T_F32 ? 16 : 8, out4 = out_type == ADKV_T_F32 ? 16 : 8;
+    if (!aligned_to(qkv, in4) || !aligned_to(q_weight, in4) || !aligned_to(k_weight, in4) || !aligned_to(q, out4) || !aligned_to(k, out4) ||
+        !aligned_to(v, out4) || !aligned_to(cos, 4) || !aligned_to(sin, 4) || !aligned_to(positions, 4))
+        return ADKV_E_ALIGN;
+    if (!positions && B && T && (long long)start + T > table_rows) return ADKV_E_CAPACITY;
+    if (B == 0 || T == 0) return 0;
+    const RopeArgs a{qkv, stride_b, stride_t, q, k, v, q_weight, k_weight, static_cast<const float *>(cos), static_cast<const float *>(sin),
+                     static_cast<const int *>(positions), table_stride, table_rows, rot, positions_per_token, start, T, Hq, Hkv, interleaved, eps};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (D) {
+    case 64: return launch_rope<64>(a, B, in_type, out_type, s);
+    case 128: return launch_rope<128>(a, B, in_type, out_type, s);
+    case 256: return launch_rope<256>(a, B, in_type, out_type, s);
+    default: return launch_rope<512>(a, B, in_type, out_type, s);
+    }
+}
+
+int adkv_process_logits(const void *x, long long stride_x, void *out, long long stride_out, int type, void *tokens, const void *history,
+                        long long stride_history, int history_cap, const void *history_lens, const void *repetition, float repetition1,
+                        const void *presence, float presence1, const void *frequency, float frequency1, const void *bias,
+                        long long stride_bias, const void *mask, long long stride_mask, int B, int V, void *stream)
+{
+    if (!x || !out) return ADKV_E_NULL;
+    if (B < 0 || V <= 0 || V > 0x7fff0000 || history_cap < 0 || B > 65535) return ADKV_E_SHAPE;
+    if (type < ADKV_T_F16 || type > ADKV_T_F32) return ADKV_E_TYPE;
+    const unsigned size = type == ADKV_T_F32 ? 4 : 2;
+    if (!aligned_to(x, size) || !aligned_to(out, size) || !aligned_to(tokens, 4) || !aligned_to(history, 4) || !aligned_to(history_lens, 4) ||
+        !aligned_to(repetition, 4) || !aligned_to(presence, 4) || !aligned_to(frequency, 4) || !aligned_to(bias, 4) || !aligned_to(mask, 4))
+        return ADKV_E_ALIGN;
+    if (B == 0) return 0;
+    const auto f = [](const void *p) { return static_cast<const float *>(p); };
+    const LogitArgs a{x, out, static_cast<int *>(tokens), static_cast<const int *>(history), static_cast<const int *>(history_lens), f(repetition),
+                      f(presence), f(frequency), repetition1, presence1, frequency1, f(bias), static_cast<const uint32_t *>(mask), stride_x,
+                      stride_out, stride_history, stride_bias, stride_mask, V, history_cap, 0};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return type == ADKV_T_F16 ? launch_logits<__half>(a, B, s) : type == ADKV_T_BF16 ? launch_logits<__nv_bfloat16>(a, B, s) : launch_logits<float>(a, B, s);
+}
+
+}  // extern "C"

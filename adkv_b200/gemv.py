@@ -29,7 +29,8 @@ from . import _lib
 
 __all__ = ["encode_kv", "forward_qk", "forward_ov", "decode_attn", "append_kv", "encode_kv_pair",
            "append_kv_pair", "n_super_for", "alloc_ckpt", "ckpt_capacity", "decode_scratch_bytes",
-           "decode_attn_varlen", "decode_attn_static", "encode_kv_layers", "append_kv_layers", "LayerSet"]
+           "decode_attn_varlen", "decode_attn_static", "encode_kv_layers", "append_kv_layers", "LayerSet",
+           "SharedPrefix", "prefix_scratch_bytes", "decode_attn_prefix"]
 
 
 def n_super_for(tokens: int, bits: int = 4) -> int:
@@ -180,10 +181,11 @@ def _tail_ptr(tail, B, H, D):
 
 def encode_kv_pair(k_cache, k_new, k_params, v_cache, v_new, v_params, scale_min, scale_max, *, bits: int = 4,
                    k_tail=None, v_tail=None, t_start: int = 0, k_ckpt=None, v_ckpt=None, ckpt_interval: int = 0,
-                   half_state: bool = False):
+                   half_state: bool = False, from_tail: bool = False):
     """``encode_kv`` for the K and V tensors of one layer in a single launch (same contract each;
     replaces the two calls of ``src/adkv/hf/llama_adkv.py:144-153``).  With ``k_ckpt`` / ``v_ckpt`` /
-    ``ckpt_interval`` every state checkpoint reached is written as well (see :func:`alloc_ckpt`)."""
+    ``ckpt_interval`` every state checkpoint reached is written as well (see :func:`alloc_ckpt`).  ``from_tail``: start from the
+    tails at ``t_start == 0`` too (the own tokens of a sequence behind a :class:`SharedPrefix`; fp32 arithmetic)."""
     _require(k_new.dtype == torch.float16 and v_new.dtype == torch.float16, "kv_new must be float16")
     B, H, n_super_cap, D = _cache_dims(k_cache, "kv_cache")
     _require(tuple(v_cache.shape) == tuple(k_cache.shape) and v_cache.dtype == torch.uint8 and v_cache.is_cuda,
@@ -201,13 +203,14 @@ def encode_kv_pair(k_cache, k_new, k_params, v_cache, v_new, v_params, scale_min
     vp, keep_v = _params(names, tuple(v_params), H, D, k_cache.device)
     xk, xv = k_new.contiguous(), v_new.contiguous()
     with _on_device(k_cache.device):
-        if half_state:
+        if half_state or from_tail:
             kc, vc, iv, cap = _ckpt_args(k_ckpt, v_ckpt, ckpt_interval, B, H, D) if ckpt_interval else (None, None, 0, 0)
             rc = _lib.load().adkv_encode_kv_flags(k_cache.data_ptr(), xk.data_ptr(), ctypes.addressof(kp),
                                                   _tail_ptr(k_tail, B, H, D), kc, v_cache.data_ptr(), xv.data_ptr(),
                                                   ctypes.addressof(vp), _tail_ptr(v_tail, B, H, D), vc, iv, cap, B, H, T,
                                                   D, n_super_cap, bits, t_start, scale_min, scale_max,
-                                                  _lib.FLAG_HALF_STATE, _stream(k_cache))
+                                                  (_lib.FLAG_HALF_STATE if half_state else 0) |
+                                                  (_lib.FLAG_TAIL_START if from_tail else 0), _stream(k_cache))
         elif ckpt_interval:
             kc, vc, iv, cap = _ckpt_args(k_ckpt, v_ckpt, ckpt_interval, B, H, D)
             rc = _lib.load().adkv_encode_kv_ckpt(k_cache.data_ptr(), xk.data_ptr(), ctypes.addressof(kp),
@@ -590,6 +593,112 @@ def decode_attn_varlen(q, k_cache, v_cache, k_new, v_new, k_params, v_params, se
                                                  _lib.flags(_fast_default(fast, k_tail), half_state, tail_keep),
                                                  _stream(k_cache))
     _lib.check(rc, "decode_attn_varlen")
+    return out
+
+
+class SharedPrefix:
+    """The packed tokens that several sequences begin with, as one K and one V cache of batch 1, for :func:`decode_attn_prefix`.
+
+    ``k_cache`` / ``v_cache`` ``[1, nh_kv, n_super, DIM/4, 4, 4]`` hold ``tokens`` tokens; ``k_tail`` / ``v_tail`` (float32 ``[1, nh_kv, 2,
+    DIM]``) are the state behind the last of them; ``k_ckpt`` / ``v_ckpt`` / ``ckpt_interval`` the state checkpoints between which the
+    prefix is replayed in parallel (all as :func:`encode_kv_pair` writes them; without checkpoints it is replayed in one piece, which a
+    long prefix pays for).  The tensors are kept and read by every step; they must not change while the prefix is in use (tokens
+    appended behind ``tokens`` do no harm)."""
+
+    def __init__(self, k_cache, v_cache, tokens: int, *, k_tail, v_tail, bits: int = 4, k_ckpt=None, v_ckpt=None, ckpt_interval: int = 0):
+        one, H, n_super_cap, D = _cache_dims(k_cache, "k_cache")
+        _require(one == 1, "a shared prefix is a cache of one sequence")
+        _require(D == 128, "a shared prefix needs head dim 128")
+        _require(bits in (2, 4), "bits must be 2 or 4")
+        _require(tuple(v_cache.shape) == tuple(k_cache.shape) and v_cache.dtype == torch.uint8 and v_cache.device == k_cache.device,
+                 "v_cache must match k_cache")
+        _require(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous")
+        _require(0 <= tokens <= n_super_cap * (32 // bits), f"the caches do not hold {tokens} tokens")
+        _require(k_tail is not None and v_tail is not None, "a shared prefix needs both tail states")
+        kt, vt = _tail_ptr(k_tail, 1, H, D), _tail_ptr(v_tail, 1, H, D)
+        kc = vc = None
+        cap = 0
+        if ckpt_interval:
+            kc, vc, _, cap = _ckpt_args(k_ckpt, v_ckpt, ckpt_interval, 1, H, D)
+            _require(max(tokens - 1, 0) // ckpt_interval <= cap, f"the checkpoints do not reach {tokens} tokens")
+        for t in (v_cache, k_tail, v_tail) + ((k_ckpt, v_ckpt) if ckpt_interval else ()):
+            _require(t.device == k_cache.device, "all tensors of a prefix must be on one CUDA device")
+        self.tokens, self.bits, self.H, self.D, self.interval, self.device = int(tokens), bits, H, D, int(ckpt_interval), k_cache.device
+        self.k_tail, self.v_tail = k_tail, v_tail
+        self._keep = (k_cache, v_cache, k_ckpt, v_ckpt)
+        self.desc = _lib.Prefix(k_cache.data_ptr(), v_cache.data_ptr(), kt, vt, kc, vc, self.tokens, n_super_cap, self.interval, cap)
+
+    def start_tails(self, B: int):
+        """Tail states ``[B, nh_kv, 2, DIM]`` of K and V for B sequences that have no tokens of their own yet."""
+        return self.k_tail.repeat(B, 1, 1, 1), self.v_tail.repeat(B, 1, 1, 1)
+
+
+def prefix_scratch_bytes(B: int, Hq: int, prefix: SharedPrefix) -> int:
+    """Scratch bytes :func:`decode_attn_prefix` needs for B sequences of Hq query heads."""
+    n = _lib.load().adkv_decode_attn_prefix_scratch_bytes(B, Hq, prefix.H, prefix.tokens, prefix.interval)
+    _lib.check(min(n, 0), "prefix_scratch_bytes")
+    return n
+
+
+def decode_attn_prefix(q, prefix: SharedPrefix, k_cache, v_cache, k_new, v_new, k_params, v_params, T, scaling: float, scale_min,
+                       scale_max, *, k_tail: torch.Tensor, v_tail: torch.Tensor, tail_keep: bool = False,
+                       out: torch.Tensor | None = None, scratch: torch.Tensor | None = None):
+    """Fused decode step of B sequences that share a packed prefix, which is replayed once for all of them.
+
+    ``k_cache`` / ``v_cache [B, nh_kv, n_super, DIM/4, 4, 4]`` hold the sequences' own tokens from index 0 on, quantised from the state
+    behind the prefix (``encode_kv_pair(..., from_tail=True)``, ``append_kv_pair``, or earlier steps); ``T`` is their number: an int, or an
+    int32 CUDA tensor ``[B]`` with one per sequence (0 or more; the caller advances it afterwards, and the step can be replayed from a
+    captured graph).  ``k_tail`` / ``v_tail`` (float32 ``[B, nh_kv, 2, DIM]``) are the states behind the last own token -- the prefix's where
+    there is none, see :meth:`SharedPrefix.start_tails` -- and advance (``tail_keep``: do not).  Queries, new tokens, parameters and result
+    as in :func:`decode_attn`: query b attends to the prefix, its own tokens and its new token, which is appended at index ``T``.
+
+    ``scratch`` (at least :func:`prefix_scratch_bytes`) is allocated per call when not given; two steps that may overlap on the GPU,
+    captured graphs among them, must not share one."""
+    _require(isinstance(prefix, SharedPrefix), "prefix must be a SharedPrefix")
+    _require(q.dtype == torch.float16, "q must be float16")
+    _require(k_new.dtype == torch.float16 and v_new.dtype == torch.float16, "k_new / v_new must be float16")
+    B, Hkv, n_super_cap, D = _cache_dims(k_cache, "k_cache")
+    bits, device = prefix.bits, k_cache.device
+    _require(tuple(v_cache.shape) == tuple(k_cache.shape) and v_cache.dtype == torch.uint8 and v_cache.is_cuda,
+             "v_cache must match k_cache")
+    _require(k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous (appended in place)")
+    _require(Hkv == prefix.H and D == prefix.D and device == prefix.device, "the caches do not match the prefix")
+    _require(q.dim() == 4 and q.shape[2] == 1 and q.shape[0] == B and q.shape[3] == D, "q must be [B, nh, 1, DIM]")
+    Hq = q.shape[1]
+    _require(Hq % Hkv == 0, "q heads must be a multiple of the cache's heads")
+    _require(k_new.numel() == B * Hkv * D and v_new.numel() == B * Hkv * D, "k_new / v_new must be [B, nh, 1, DIM]")
+    lens = None
+    if isinstance(T, torch.Tensor):
+        _require(T.dtype == torch.int32 and T.is_cuda and T.device == device and T.is_contiguous() and T.numel() == B,
+                 "T must be an int or a contiguous int32 CUDA tensor with one entry per sequence")
+        lens, T = T.data_ptr(), 0
+    _require(T >= 0, "T must be non-negative")
+    _require(T // (32 // bits) < n_super_cap, f"cache has no free supergroup to append token {T}")
+    _require(k_tail is not None and v_tail is not None, "a step behind a prefix needs both tail states")
+    kt, vt = _tail_ptr(k_tail, B, Hkv, D), _tail_ptr(v_tail, B, Hkv, D)
+    for t in (q, k_new, v_new, v_cache, k_tail, v_tail):
+        _require(t.device == device, "all tensors must be on the cache's CUDA device")
+    names = ("zp", "sc", "alpha", "beta", "t")
+    kp, keep_k = _params(tuple("k_" + n for n in names), tuple(k_params), Hkv, D, device)
+    vp, keep_v = _params(tuple("v_" + n for n in names), tuple(v_params), Hkv, D, device)
+    qc, kn, vn = q.contiguous(), k_new.contiguous(), v_new.contiguous()
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float16, device=device)
+    else:
+        _require(out.dtype == torch.float16 and out.is_contiguous() and out.shape == (B, Hq, D) and out.device == device,
+                 "out must be contiguous float16 [B, nh_q, DIM]")
+    if B == 0:
+        return out
+    with _on_device(device):
+        if scratch is None:
+            scratch = torch.empty(prefix_scratch_bytes(B, Hq, prefix), dtype=torch.uint8, device=device)
+        _require(scratch.is_contiguous() and scratch.device == device, "scratch must be a contiguous CUDA tensor")
+        rc = _lib.load().adkv_decode_attn_prefix(qc.data_ptr(), ctypes.addressof(prefix.desc), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                 kn.data_ptr(), vn.data_ptr(), ctypes.addressof(kp), ctypes.addressof(vp), kt, vt, lens, T,
+                                                 out.data_ptr(), scratch.data_ptr(), scratch.numel() * scratch.element_size(), B, Hq, Hkv,
+                                                 D, n_super_cap, bits, scaling, scale_min, scale_max, _lib.flags(True, tail_keep=tail_keep),
+                                                 _stream(k_cache))
+    _lib.check(rc, "decode_attn_prefix")
     return out
 
 

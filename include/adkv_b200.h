@@ -49,6 +49,8 @@ extern "C" {
 #define ADKV_E_FLAGS     (-10) /* a flag or optional argument is not available in this combination (tail states with
                                   ADKV_FLAG_HALF_STATE; only one of the two tail states given) */
 
+#define ADKV_E_TYPE      (-11) /* element types not available in this combination */
+
 /* Size of the library's built-in scratch array (see adkv_decode_attn_ckpt_static). */
 #define ADKV_STATIC_SCRATCH_BYTES (16u << 20)
 
@@ -93,6 +95,10 @@ extern "C" {
  * The segments of adkv_decode_attn_ckpt take the tensor cores by the same line. */
 #define ADKV_FLAG_SPLIT_CHANNELS 8u
 #define ADKV_FLAG_NO_SPLIT_CHANNELS 16u
+/* adkv_encode_kv_flags with t_start = 0: start from the tail states, as a chunk at t_start > 0 does, instead of the initial parameters
+ * (fp32 arithmetic; ADKV_E_START without tails).  For the cache of a sequence that goes on behind a shared prefix: it holds only the
+ * sequence's own tokens, from index 0 on, and its tails begin as a copy of the prefix's. */
+#define ADKV_FLAG_TAIL_START 32u
 /* Self-test of the failure path of adkv_decode_attn_ckpt (no counterpart in the reference): the K warps return at
  * once, so whatever waits for logits waits for ever.  Each wait gives up after its 1 s limit (the tensor cores' kernel counts it
  * in cycles, 2e9), the kernels end normally, adkv_device_status reports a wait that ran out (3, or 1 to 4 of that kernel), nothing
@@ -280,9 +286,71 @@ int adkv_decode_attn_ckpt_static(const void *q, void *k_cache, void *v_cache, co
                                  int B, int Hq, int Hkv, int T, int D, int n_super_cap, int bits, float scaling,
                                  float scale_min, float scale_max, unsigned flags, void *stream);
 
+/* ---- A batch of sequences that begin with the same tokens (no counterpart in the reference, whose cache object holds every
+ * sequence whole).  The packed prefix exists once: */
+typedef struct adkv_prefix {
+    const void *k_cache, *v_cache;   /* uint32 [Hkv, n_super_cap, D], tokens [0, tokens) valid */
+    const void *k_tail, *v_tail;     /* float [Hkv, 2, D]: the state behind the last token */
+    const void *k_ckpt, *v_ckpt;     /* float [Hkv, n_ckpt_cap, 2, D] as adkv_encode_kv_ckpt writes them; needed for tokens > interval > 0 */
+    int tokens, n_super_cap;
+    int interval, n_ckpt_cap;        /* tokens between checkpoints, a multiple of 32; 0: none, the prefix is replayed in one piece */
+} adkv_prefix;
+
+/* Bytes of scratch adkv_decode_attn_prefix needs (negative: ADKV_E_*). */
+long long adkv_decode_attn_prefix_scratch_bytes(int B, int Hq, int Hkv, int prefix_tokens, int interval);
+
+/* Decode step of B sequences behind one prefix: query b attends to the prefix, to the tokens that sequence b has cached itself and to
+ * its new token, which is appended.  Same result as adkv_decode_attn_varlen with tail states and ADKV_FLAG_FAST_REPLAY on caches that
+ * hold prefix and own tokens in one piece, up to summation order and the rounding of the prefix's dequantised values to fp16 (as
+ * differences from the zero points at the start of a run of intervals, in units of 16: values are in range up to 2^20).
+ *   k_cache, v_cache  uint32 [B, Hkv, n_super_cap, D]: the sequences' own tokens, from index 0 on.  The recurrence enters them with the
+ *          state behind the prefix (prefix->k_tail, v_tail); fill them with ADKV_FLAG_TAIL_START, or with adkv_append_kv from T = 0 on.
+ *   k_tail, v_tail    float [B, Hkv, 2, D], required, in/out: the state behind the last own token, the prefix's where there is none.
+ *   seq_lens          int32 [B] on the device: own tokens of each sequence, 0 or more; or NULL: T of each.  A length that does not fit
+ *          the cache is reported by adkv_device_status (6): nothing is appended, the outputs of that sequence are NaN.
+ *   scratch           at least adkv_decode_attn_prefix_scratch_bytes, 16-byte aligned, contents irrelevant; not for two calls at once.
+ * Head dim 128, Hq / Hkv of 1, 2, 4 or 8; flags: ADKV_FLAG_TAIL_KEEP (ADKV_FLAG_FAST_REPLAY is implied). */
+int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
+                            const adkv_params *kp, const adkv_params *vp, void *k_tail, void *v_tail, const void *seq_lens, int T,
+                            void *out, void *scratch, long long scratch_bytes, int B, int Hq, int Hkv, int D, int n_super_cap, int bits,
+                            float scaling, float scale_min, float scale_max, unsigned flags, void *stream);
+
+/* ---- What a step does around the attention.  Element types: */
+#define ADKV_T_F16  0
+#define ADKV_T_BF16 1
+#define ADKV_T_F32  2
+
+/* Queries, keys and values from the projection into the layout that the caches take, queries and keys normalised per head and rotated
+ * on the way (the reference does this in torch: src/adkv/hf/llama_adkv.py:333-345).
+ *   qkv   [B, T, (Hq + 2 Hkv) * D] of in_type, sequences stride_b and tokens stride_t elements apart (multiples of 4)
+ *   q [B, Hq, T, D], k, v [B, Hkv, T, D]  contiguous, of out_type: in_type or fp16; v is copied
+ *   q_weight, k_weight  [D] of in_type, or NULL: x / sqrt(mean(x^2) + eps) * weight before the rotation
+ *   cos, sin  float [table_rows, rot / 2], rows table_stride elements apart, row = position; rot is a multiple of 8, at most D; channels
+ *         from rot on pass through.  Pairs are (i, i + rot / 2), or (2i, 2i + 1) if interleaved.
+ *   positions int32 on the device, [B] (of each first token) or, with positions_per_token, [B, T]; NULL: start + t.  A position without
+ *         a row cannot be rejected on the host: adkv_device_status reports 8, q and k of that token are NaN.
+ * fp32 arithmetic, rounded once at the end.  D = 64, 128, 256 or 512; pointers aligned to four elements. */
+int adkv_norm_rope_qkv(const void *qkv, long long stride_b, long long stride_t, int in_type, void *q, void *k, void *v, int out_type,
+                       const void *q_weight, const void *k_weight, float eps, const void *cos, const void *sin, long long table_stride,
+                       int table_rows, int rot, const void *positions, int positions_per_token, int start, int B, int T, int Hq, int Hkv,
+                       int D, int interleaved, void *stream);
+
+/* Logits [B, V] under penalties, biases and masks, and the choice of the next token (no counterpart in the reference).
+ *   n = how often the token is in history[b, 0 .. history_lens[b]) (int32 ids; those outside [0, V) do not count; history_lens NULL:
+ *   history_cap of each).  n > 0: x = x > 0 ? x / repetition : x * repetition, then x - (frequency * n + presence).
+ *   Then + bias (float [V] with stride_bias 0, or [B, V]), and -inf where bit v % 32 of mask[b, v / 32] (uint32) is not set.
+ *   repetition, presence, frequency: float [B], or NULL: the number that follows.
+ *   out  of the logits' type, may be the logits; tokens int32 [B] or NULL: the lowest index of the largest element of out (a NaN counts
+ *         as the largest), -1 where every element is -inf.
+ * fp32 arithmetic, rounded once at the end; rows need no alignment beyond their type's; B at most 65535. */
+int adkv_process_logits(const void *x, long long stride_x, void *out, long long stride_out, int type, void *tokens, const void *history,
+                        long long stride_history, int history_cap, const void *history_lens, const void *repetition, float repetition1,
+                        const void *presence, float presence1, const void *frequency, float frequency1, const void *bias,
+                        long long stride_bias, const void *mask, long long stride_mask, int B, int V, void *stream);
+
 /* Reads and clears the device-side status word of the current device (HOST pointer `status`;
 * synchronises `stream`).  Non-zero means a kernel gave up on a bounded wait (1-5: which wait) or skipped a
- * stream whose device-side length did not fit the cache (6).  Intended for tests and diagnostics, not for the hot path. */
+ * stream whose device-side length did not fit the cache (6), or met a device-side position without a row in the tables (8).  Intended for tests and diagnostics, not for the hot path. */
 int adkv_device_status(int *status, void *stream);
 
 /* Self-test of the bounded waits (no counterpart in the reference): launches one warp that waits on a barrier
