@@ -16,6 +16,8 @@
 // of two, so that differences up to a million are in range.  Weights are rounded to fp16, sums of both products are fp32.
 #include "adkv_host.h"
 
+#include <algorithm>
+
 #include "adkv_softmax.cuh"
 #include "adkv_tensor.cuh"
 
@@ -33,19 +35,33 @@ struct PrefixArgs {
     const float *ckpt[2];            // [Hkv, n_ckpt_cap, 2, kD]; entry i = state before token (i + 1) * interval
     ParamPtrs p[2];
     float *scratch;                  // [B * Hkv, n_parts, G, kPartStride]
-    int Hq, Hkv, rows, row_tiles, n_super_cap, n_ckpt_cap, tokens, interval;
-    int run, n_runs, n_parts;        // tokens of a run (a multiple of interval), runs, parts of a stream in scratch
+    int Hq, Hkv, rows, n_super_cap, n_ckpt_cap, tokens;
     float scaling, smin, smax;
 };
 
+// How the prefix is laid over CTAs.  The intervals of all units (128 rows of one head) form one line, of which every CTA takes an equal
+// piece: whole intervals, so that it can enter anywhere.  A piece that crosses from one unit to the next is two runs.
+struct PrefixPlan {
+    int n_int, interval, row_tiles, ctas, n_parts;   // intervals of a unit, their tokens; n_parts: room for the runs of a unit
+    long long n;                                     // intervals of all units
+    __host__ __device__ long long first(int cta) const { return n * cta / ctas; }
+    __host__ __device__ int cta_of(long long at) const { return int(((at + 1) * ctas - 1) / n); }
+};
+
+template <int BITS>
 struct PrefixShared {
     alignas(128) __half q[kD / 8][kPreRows][8];          // [channel / 8][row][channel % 8]
     alignas(128) __half x[2][2][kPreTok / 8][kD][8];     // K, V; buffer; [token / 8][channel][token % 8]
+    alignas(128) uint32_t words[2][2][kPreTok * BITS / 32][kD];   // packed tiles of K and V
     float z0[kD];                                        // zero points of K before the run
+    // The results of the run lie in x and what follows, a row every kPartStride floats (no two of eight in the same banks), and the zero
+    // points of V before the run in the last row of words, where only their own thread has read.
+    __device__ float *row(int r) { return reinterpret_cast<float *>(&x[0][0][0][0][0]) + r * kPartStride; }
+    __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][1][kPreTok * BITS / 32 - 1][0]); }
     uint32_t tmem;
     int dead;                                            // a bounded wait gave up
-    // of tile i, buffer i % 2: K and V values are there; S is there (and K has been read); weights are there; O is added up (V, P read)
-    uint64_t full[2][2], sdone[2], pfull[2], odone[2];
+    // of tile i, buffer i % 2: words are there; K and V values are there; S is there (and K has been read); weights are there; O is added up (V, P read)
+    uint64_t loaded[2][2], full[2][2], sdone[2], pfull[2], odone[2];
 };
 
 // K-major shared-memory matrix without swizzle: element (m, k) lies at (m / 8) * m_stride + (k / 8) * k_stride + (m % 8) * 16 + (k % 8) * 2.
@@ -56,38 +72,41 @@ __host__ __device__ constexpr uint32_t pre_mma_desc(int M, int N, bool b_mn)
     return 1u << 4 | uint32_t(b_mn) << 16 | uint32_t(N >> 3) << 17 | uint32_t(M >> 4) << 24;
 }
 
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 // What one thread keeps of its channel, in units of kPreUnit; the zero point counts from the start of the run.
 struct PrefixChan {
-    float zp, s, alpha, beta, tc, lo, hi;   // lo, hi: scales that eight updates cannot bring to a bound
-    __device__ __forceinline__ bool safe() const { return __all_sync(kFull, s >= lo && s <= hi); }
+    float zp, s, alpha, beta, tc;
 };
-// Eight tokens, fields 0..7 of w, contracted as in k_chunk2.
+// Eight tokens, fields 0..7 of w, contracted as in k_chunk2; the values go to dst.
 template <int BITS, bool GUARDED>
-__device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS> &fc, PrefixChan &c, float smin, float smax, float eps, float (&x)[8])
+__device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS> &fc, PrefixChan &c, float smin, float smax, float eps, int left, uint8_t *dst)
 {
+    float x[8];
     static_for<8>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
         const float q = fc.template code<j % 4>(j < 4 ? w : w >> (4 * BITS));
         const float rh = __fmul_rn(q, GUARDED ? fmaxf(c.s, eps) : c.s);
         x[j] = __fadd_rn(rh, c.zp);
+        if (GUARDED && j >= left) x[j] = 0.f;   // behind the last token: whatever the words hold there does not count
         c.zp = fmaf(c.alpha, rh, c.zp);
         c.s *= fmaf(c.beta, fabsf(q), c.tc);
         if (GUARDED) c.s = fminf(fmaxf(c.s, smin), smax);
     });
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
 }
-struct PrefixWindow {
-    float x[8], zp, s;
-};
+// The guarded and the ragged window, by a call that keeps them out of the loop and of its registers.
 template <int BITS>
-__device__ __noinline__ PrefixWindow prefix_window_guarded(uint32_t w, PrefixChan c, float smin, float smax, float eps)
+__device__ __noinline__ float2 prefix_window_guarded(uint32_t w, PrefixChan c, float smin, float smax, int left, uint8_t *dst)
 {
     FieldConsts<BITS> fc;
     fc.init();
-    PrefixWindow r;
-    prefix_window<BITS, true>(w, fc, c, smin, smax, eps, r.x);
-    r.zp = c.zp;
-    r.s = c.s;
-    return r;
+    prefix_window<BITS, true>(w, fc, c, smin * (1.f / kPreUnit), smax * (1.f / kPreUnit), kEps * (1.f / kPreUnit), left, dst);
+    return make_float2(c.zp, c.s);
 }
 
 __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreSlack
@@ -96,35 +115,33 @@ __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane)
+__device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane, int count = 1)
 {
     __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+// A row of results goes to scratch as one copy of its own thread, once that thread's writes can be seen by the copy engine.
+__device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)), "r"(smem_u32(src)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_constant__ PrefixArgs a)
+__global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_constant__ PrefixArgs a, const __grid_constant__ PrefixPlan plan)
 {
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    PrefixShared &sh = *reinterpret_cast<PrefixShared *>(smem_raw);
-    constexpr int TPW = Codec<BITS>::TPW, ROWS = kPreTok / TPW;                 // word rows of a tile
+    PrefixShared<BITS> &sh = *reinterpret_cast<PrefixShared<BITS> *>(smem_raw);
+    constexpr int TPW = Codec<BITS>::TPW, WORDS = kPreTok / TPW;                // word rows of a tile
     constexpr uint32_t kColS = 0, kColO = 2 * kPreTok, kColumns = 256;          // S (and P in its place) twice, O
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles % a.Hkv, run = blockIdx.x / a.row_tiles / a.Hkv;
     const int G = a.Hq / a.Hkv;
-    const int t0 = run * a.run, ntok = min(a.run, a.tokens - t0), n_tiles = (ntok + kPreTok - 1) / kPreTok;
-    const int n_rows = (ntok + TPW - 1) / TPW;                                  // word rows of the run
-    const int rows = min(kPreRows, a.rows - rt * kPreRows);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the sequences' own tokens may be scanned beside this kernel
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.loaded[0][i], 1);
+            mbar_init(&sh.loaded[1][i], 1);
             mbar_init(&sh.full[0][i], 4);
             mbar_init(&sh.full[1][i], 4);
             mbar_init(&sh.sdone[i], 1);
@@ -135,269 +152,372 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         mbar_init_fence();
     }
     if (warp == 12) tmem_alloc(&sh.tmem, kColumns);
-    // query rows, negated where the scaling is negative (rows behind the last one as zeros)
-    const uint32_t sign = a.scaling < 0.f ? 0x80008000u : 0u;
-    for (int i = threadIdx.x; i < kPreRows * (kD / 8); i += kPreThreads) {
-        const int r = i / (kD / 8), k = i % (kD / 8), n = rt * kPreRows + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-            const uint2 *src = reinterpret_cast<const uint2 *>(a.q + (size_t(n / G) * a.Hq + size_t(h) * G + n % G) * kD + 8 * k);
-            const uint2 lo = src[0], hi = src[1];
-            v = make_uint4(lo.x ^ sign, lo.y ^ sign, hi.x ^ sign, hi.y ^ sign);
-        }
-        *reinterpret_cast<uint4 *>(&sh.q[k][r][0]) = v;
-    }
-    const int which = warp >> 2 & 1;   // of the scanning warps: 0 K, 1 V
-    const int c = threadIdx.x & (kD - 1);
-    PrefixChan ch;
-    float start = 0.f;                 // zero point before the run: K, and V for the threads that store the result
-    if (warp < 8) {
-        const ParamPtrs &p = a.p[which];
-        const size_t po = size_t(h) * kD + c;
-        const float alpha = __half2float(p.alpha[po]), beta = __half2float(p.beta[po]), target = __half2float(p.target[po]);
-        float s;
-        if (t0 > 0) {
-            const float *init = a.ckpt[which] + (size_t(h) * a.n_ckpt_cap + t0 / a.interval - 1) * 2 * kD;
-            start = init[c];
-            s = init[kD + c];
-        } else {
-            start = __half2float(p.zp_init[po]);
-            s = __half2float(p.scale_init[po]);
-        }
-        if (which == 0) sh.z0[c] = start;
-        SafeRange safe{0.f, INFINITY};
-        const float be[1] = {beta}, tg[1] = {target};
-        safe.template init<BITS, 1>(be, tg, a.smin, a.smax);
-        ch = PrefixChan{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f), safe.lo * (1.f / kPreUnit), safe.hi * (1.f / kPreUnit)};
-    }
-    fence_async_shared();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    const int which = warp >> 2 & 1;   // of the scanning warps: 0 K, 1 V
+    const int c = threadIdx.x & (kD - 1);
+    const float scale2 = a.scaling * 1.4426950408889634f;
+    const int log_g = __ffs(G) - 1;    // 1, 2, 4 or 8 heads
     bool ok = true;
+    int done = 0;                      // tiles of the runs so far
 
-    if (warp < 8) {
-        // ------------------------------------------------------------------------------ K and V values
-        FieldConsts<BITS> fc;
-        fc.init();
-        const uint32_t *words = reinterpret_cast<const uint32_t *>(a.cache[which]) + (size_t(h) * a.n_super_cap + t0 / TPW) * kD + c;
-        const float smin = a.smin * (1.f / kPreUnit), smax = a.smax * (1.f / kPreUnit), eps = kEps * (1.f / kPreUnit);
-        uint64_t *freed = which ? sh.odone : sh.sdone;
-        uint32_t next[ROWS];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) next[r] = r < n_rows ? words[size_t(r) * kD] : 0u;
-        bool safe = ch.safe();
+    const long long last = plan.first(blockIdx.x + 1);
 #pragma unroll 1
-        for (int i = 0; i < n_tiles; ++i) {
-            const int buf = i & 1;
-            uint32_t w[ROWS];
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) w[r] = next[r];
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) next[r] = (i + 1) * ROWS + r < n_rows ? words[size_t((i + 1) * ROWS + r) * kD] : 0u;
-            if (i >= 2 && !(ok = mbar_wait(&freed[buf], (i / 2 & 1) ^ 1, kStatKWait))) break;
-            uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][buf][0][c][0]);
-            const int left = ntok - i * kPreTok;
-#pragma unroll
-            for (int n = 0; n < kPreTok / 8; ++n) {
-                const uint32_t word = BITS == 4 ? w[n % ROWS] : w[n / 2 % ROWS] >> (16 * (n & 1));
-                float x[8];
-                if (safe) {
-                    prefix_window<BITS, false>(word, fc, ch, smin, smax, eps, x);
-                } else {
-                    const PrefixWindow r = prefix_window_guarded<BITS>(word, ch, smin, smax, eps);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = r.x[j];
-                    ch.zp = r.zp;
-                    ch.s = r.s;
+    for (long long at = plan.first(blockIdx.x); at < last;) {
+        // ------------------------------------------------------------------------------ a run: intervals i0 .. i1 of a unit
+        const int unit = int(at / plan.n_int), i0 = int(at % plan.n_int), i1 = int(min((long long)plan.n_int, i0 + last - at));
+        at += i1 - i0;
+        const int rt = unit % plan.row_tiles, h = unit / plan.row_tiles;
+        const int t0 = i0 * plan.interval, ntok = min(a.tokens, i1 * plan.interval) - t0, n_tiles = (ntok + kPreTok - 1) / kPreTok;
+        const int rows = min(kPreRows, a.rows - rt * kPreRows);
+        // packed tile i of K or V, by one lane of a warp
+        const auto load_tile = [&](int tensor, int i) {
+            const int tile = done + i, n = min(WORDS, (ntok + TPW - 1) / TPW - i * WORDS);
+            uint64_t *bar = &sh.loaded[tensor][tile & 1];
+            mbar_expect_tx(bar, n * kD * 4);
+            bulk_load(&sh.words[tensor][tile & 1][0][0], a.cache[tensor] + (size_t(h) * a.n_super_cap + t0 / TPW + size_t(i) * WORDS) * kD * 4,
+                      n * kD * 4, bar);
+        };
+
+        // Query rows, negated where the scaling is negative (rows behind the last one as zeros), by the six warps that are not scanning.
+        const auto load_q = [&](int thread) {
+            const uint32_t sign = a.scaling < 0.f ? 0x80008000u : 0u;
+            constexpr int THREADS = kPreThreads - 256, N = kPreRows * (kD / 8);
+            const auto load = [&](int i) {
+                const int r = i / (kD / 8), k = i % (kD / 8), n = rt * kPreRows + r;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (i < N && r < rows) {
+                    const uint2 *src = reinterpret_cast<const uint2 *>(a.q + (size_t(n >> log_g) * a.Hq + (size_t(h) << log_g) + (n & (G - 1))) * kD + 8 * k);
+                    const uint2 x = src[0], y = src[1];
+                    v = make_uint4(x.x ^ sign, x.y ^ sign, y.x ^ sign, y.y ^ sign);
                 }
-                safe = ch.safe();
-                if (left < 8 * n + 8) {   // behind the last token: whatever the words hold there does not count
+                return v;
+            };
+#pragma unroll 1
+            for (int i = thread; i < N; i += 4 * THREADS) {
+                uint4 v[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = 8 * n + j < left ? x[j] : 0.f;
+                for (int u = 0; u < 4; ++u) v[u] = load(i + u * THREADS);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int at = i + u * THREADS;
+                    if (at < N) *reinterpret_cast<uint4 *>(&sh.q[at % (kD / 8)][at / (kD / 8)][0]) = v[u];
                 }
-                *reinterpret_cast<uint4 *>(dst + n * kD * 16) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
             }
             fence_async_shared();
-            warp_arrive(&sh.full[which][buf], lane);
-        }
-        if (!ok && lane == 0) sh.dead = 1;
-        __syncthreads();
-    } else if (warp < 12) {
-        // ------------------------------------------------------------------------------ weights, a row a thread
-        const int e = warp & 3, r = 32 * e + lane;
-        const bool busy = 32 * e < rows;
-        const uint32_t lanes = tmem + (uint32_t(32 * e) << 16);
-        const float scale2 = a.scaling * 1.4426950408889634f, f = fabsf(scale2) * kPreUnit;
-        float m = -INFINITY, l = 0.f;
+            asm volatile("bar.sync 1, 192;" ::: "memory");
+        };
+
+        if (warp < 8) {
+            // -------------------------------------------------------------------------- K and V values
+            FieldConsts<BITS> fc;
+            fc.init();
+            const ParamPtrs &p = a.p[which];
+            const size_t po = size_t(h) * kD + c;
+            const float alpha = __half2float(p.alpha[po]), beta = __half2float(p.beta[po]), target = __half2float(p.target[po]);
+            float s, start;
+            if (i0 > 0) {
+                const float *init = a.ckpt[which] + (size_t(h) * a.n_ckpt_cap + i0 - 1) * 2 * kD;
+                start = init[c];
+                s = init[kD + c];
+            } else {
+                start = __half2float(p.zp_init[po]);
+                s = __half2float(p.scale_init[po]);
+            }
+            SafeRange safe{0.f, INFINITY};
+            const float be[1] = {beta}, tg[1] = {target};
+            safe.template init<BITS, 1>(be, tg, a.smin, a.smax);
+            const float lo = safe.lo * (1.f / kPreUnit), hi = safe.hi * (1.f / kPreUnit);   // scales that eight updates cannot bring to a bound
+            PrefixChan ch{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f)};
+            if (which == 0) sh.z0[c] = start;
+            uint64_t *freed = which ? sh.odone : sh.sdone;
 #pragma unroll 1
-        for (int i = 0; i < n_tiles; ++i) {
-            const int buf = i & 1;
-            if (!(ok = mbar_wait(&sh.sdone[buf], i / 2 & 1, kStatLFullWait))) break;
-            if (busy) {
-                tc_fence_after();
-                const uint32_t at = lanes + kColS + kPreTok * buf;
-                const int left = ntok - i * kPreTok;
-                float top = -INFINITY;
+            for (int i = 0; i < n_tiles; ++i) {
+                const int tile = done + i, buf = tile & 1;
+                // the words have come, and the products that read this buffer before are done
+                if (!(ok = mbar_wait_both(&sh.loaded[which][buf], tile >> 1 & 1, tile >= 2 ? &freed[buf] : nullptr, (tile >> 1 & 1) ^ 1, kStatKWait))) break;
+                const uint32_t *row = &sh.words[which][buf][0][c];
+                uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][buf][0][c][0]);
+                int left = ntok - i * kPreTok;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half, left -= kPreTok / 2) {
+                    uint32_t w[WORDS / 2];
 #pragma unroll
-                for (int n = 0; n < kPreTok; n += 16) {
-                    uint32_t v[16];
-                    tmem_ld(v, at + n);
-                    tmem_wait_ld(v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) top = fmaxf(top, n + j < left ? __uint_as_float(v[j]) : -INFINITY);
+                    for (int k = 0; k < WORDS / 2; ++k, row += kD) w[k] = *row;
+                    static_for<kPreTok / 16>([&](auto nc) {
+                        constexpr int n = decltype(nc)::value;
+                        const uint32_t word = BITS == 4 ? w[n % (WORDS / 2)] : w[n / 2 % (WORDS / 2)] >> (16 * (n & 1));
+                        if (__all_sync(kFull, ch.s >= lo && ch.s <= hi) && left >= 8 * n + 8) {
+                            prefix_window<BITS, false>(word, fc, ch, 0.f, 0.f, 0.f, 0, dst);
+                        } else {
+                            const float2 state = prefix_window_guarded<BITS>(word, ch, a.smin, a.smax, left - 8 * n, dst);
+                            ch.zp = state.x;
+                            ch.s = state.y;
+                        }
+                        dst += kD * 16;
+                    });
                 }
-                top *= f;
-                const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
-                if (__any_sync(kFull, grown)) {
-                    const float corr = grown ? exp2_fast(m - top) : 1.f;
-                    if (i > 0) {
-                        // all sums so far are in: O can be changed
-                        if (!(ok = mbar_wait(&sh.odone[buf ^ 1], ((i - 1) / 2 & 1), kStatVWait))) break;
-                        tc_fence_after();
+                fence_async_shared();
+                warp_arrive(&sh.full[which][buf], lane);
+            }
+            if (which == 1) sh.z0_v()[c] = start;
+            if (!ok && lane == 0) sh.dead = 1;
+            __syncthreads();
+        } else if (warp < 12) {
+            // -------------------------------------------------------------------------- weights, a row a thread
+            const int e = warp & 3, r = 32 * e + lane;
+            const bool busy = 32 * e < rows;
+            const uint32_t lanes = tmem + (uint32_t(32 * e) << 16);
+            const float f = fmaxf(fabsf(scale2) * kPreUnit, 1e-30f);   // not 0: masked columns are -inf times this
+            const int idle = e == 0 ? 4 - (rows + 31) / 32 : 0;        // warps without rows do not take part; the first arrives for them
+            float m = -INFINITY, l = 0.f, base = 0.f;
+            load_q(threadIdx.x - 256);
 #pragma unroll 1
-                        for (int n = 0; n < kD; n += 16) {
+            for (int i = 0; i < n_tiles && busy; ++i) {
+                const int tile = done + i, buf = tile & 1;
+                if (!(ok = mbar_wait(&sh.sdone[buf], tile >> 1 & 1, kStatLFullWait))) break;
+                {
+                    tc_fence_after();
+                    const uint32_t cols = lanes + kColS + kPreTok * buf;
+                    const int left = ntok - i * kPreTok;
+                    uint32_t p[kPreTok / 2];
+                    float top, sum;
+                    // weights with the maximum so far, and the largest column; all columns are read before the first weight is written
+                    const auto weigh = [&](auto whole) {
+                        top = -INFINITY;
+                        sum = 0.f;
+#pragma unroll
+                        for (int n = 0; n < kPreTok; n += 16) {
                             uint32_t v[16];
-                            tmem_ld(v, lanes + kColO + n);
+                            tmem_ld(v, cols + n);
                             tmem_wait_ld(v);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
-#pragma unroll
-                            for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            for (int j = 0; j < 16; j += 2) {
+                                float s0 = __uint_as_float(v[j]), s1 = __uint_as_float(v[j + 1]);
+                                if (!decltype(whole)::value) {
+                                    s0 = n + j < left ? s0 : -INFINITY;
+                                    s1 = n + j + 1 < left ? s1 : -INFINITY;
+                                }
+                                top = fmaxf(fmaxf(top, s0), s1);
+                                const float p0 = exp2_fast(fmaf(s0, f, -m)), p1 = exp2_fast(fmaf(s1, f, -m));
+                                sum += p0 + p1;
+                                p[(n + j) / 2] = pack2(p0, p1);
+                            }
                         }
+                        top *= f;
+                    };
+#pragma unroll 1
+                    for (;;) {
+                        if (left >= kPreTok) weigh(std::true_type{});
+                        else weigh(std::false_type{});
+                        const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
+                        if (!__any_sync(kFull, grown)) break;
+                        const float corr = grown ? exp2_fast(m - top) : 1.f;
+                        if (i > 0) {
+                            // all sums so far are in: O can be changed
+                            if (!(ok = mbar_wait(&sh.odone[buf ^ 1], (tile - 1) >> 1 & 1, kStatVWait))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int n = 0; n < kD; n += 16) {
+                                uint32_t v[16];
+                                tmem_ld(v, lanes + kColO + n);
+                                tmem_wait_ld(v);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
+#pragma unroll
+                                for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            }
+                        }
+                        l *= corr;
+                        if (grown) m = top;
                     }
-                    l *= corr;
-                    if (grown) m = top;
+                    if (!ok) break;
+                    l += sum;
+#pragma unroll
+                    for (int j = 0; j < kPreTok / 2; j += 4) tmem_st4(cols + j, p[j], p[j + 1], p[j + 2], p[j + 3]);
+                    tmem_wait_st();
+                    tc_fence_before();
                 }
-#pragma unroll
-                for (int n = 0; n < kPreTok; n += 16) {
-                    uint32_t v[16];
-                    tmem_ld(v, at + n);
-                    tmem_wait_ld(v);
-                    float p[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        p[j] = exp2_fast(fmaf(__uint_as_float(v[j]), f, -m));
-                        if (n + j >= left) p[j] = 0.f;
-                        l += p[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; j += 8)
-                        tmem_st4(at + (n + j) / 2, pack2(p[j], p[j + 1]), pack2(p[j + 2], p[j + 3]), pack2(p[j + 4], p[j + 5]), pack2(p[j + 6], p[j + 7]));
-                }
-                tmem_wait_st();
-                tc_fence_before();
+                warp_arrive(&sh.pfull[buf], lane, 1 + idle);
             }
-            warp_arrive(&sh.pfull[buf], lane);
-        }
-        if (ok) ok = mbar_wait(&sh.odone[(n_tiles - 1) & 1], (n_tiles - 1) / 2 & 1, kStatVWait);
-        if (!ok && lane == 0) sh.dead = 1;
-        __syncthreads();
-        const bool dead = sh.dead != 0;
-        if (busy) {
-            tc_fence_after();
-            const int n_row = rt * kPreRows + r, b = n_row / G, g = n_row % G;
-            float *part = a.scratch + ((size_t(b * a.Hkv + h) * a.n_parts + run) * G + g) * kPartStride;
-            float base = 0.f;   // what the zero points before the run add to every logit of the row
+            const int end = done + n_tiles - 1;
+            if (ok && busy) ok = mbar_wait(&sh.odone[end & 1], end >> 1 & 1, kStatVWait);
+            if (!ok && lane == 0) sh.dead = 1;
+            __syncthreads();
+            const bool dead = sh.dead != 0;
+            if (busy) {
+                tc_fence_after();
+                const int n_row = rt * kPreRows + r;
+                const int slot = blockIdx.x - plan.cta_of((long long)unit * plan.n_int);
+                float *part = a.scratch + ((size_t(n_row >> log_g) * a.Hkv + h) * plan.n_parts + slot) * (kPartStride << log_g) + (n_row & (G - 1)) * kPartStride;
+                float *row = sh.row(r);
+                // what the zero points before the run add to every logit of the row
 #pragma unroll 4
-            for (int k = 0; k < kD / 8; ++k) {
-                float qv[4];
-                load_half4(qv, &sh.q[k][r][0]);
+                for (int k = 0; k < kD / 8; ++k) {
+                    float qv[4];
+                    load_half4(qv, &sh.q[k][r][0]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + j], base);
-                load_half4(qv, &sh.q[k][r][4]);
+                    for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + j], base);
+                    load_half4(qv, &sh.q[k][r][4]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + 4 + j], base);
-            }
-            if (r < rows) {
-                part[0] = dead ? -INFINITY : fmaf(base, fabsf(scale2), m);
-                part[1] = dead ? __int_as_float(0x7fc00000) : l;
-            }
-            const float *init = a.ckpt[1] + (size_t(h) * a.n_ckpt_cap + (t0 > 0 ? t0 / a.interval - 1 : 0)) * 2 * kD;
+                    for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + 4 + j], base);
+                }
+                *reinterpret_cast<float4 *>(row) = dead ? make_float4(-INFINITY, __int_as_float(0x7fc00000), 0.f, 0.f)
+                                                        : make_float4(fmaf(base, fabsf(scale2), m), l, 0.f, 0.f);
 #pragma unroll 1
-            for (int n = 0; n < kD; n += 16) {
-                uint32_t v[16];
-                tmem_ld(v, lanes + kColO + n);
-                tmem_wait_ld(v);
-                if (r < rows) {
+                for (int n = 0; n < kD; n += 32) {
+                    uint32_t v[2][16];
+                    tmem_ld(v[0], lanes + kColO + n);
+                    tmem_ld(v[1], lanes + kColO + n + 16);
+                    tmem_wait_ld(v[0]);
+                    tmem_wait_ld(v[1]);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        float z[4];
-                        if (t0 > 0) {
-                            const float4 z4 = *reinterpret_cast<const float4 *>(init + n + j);
-                            z[0] = z4.x; z[1] = z4.y; z[2] = z4.z; z[3] = z4.w;
-                        } else {
-                            load_half4(z, a.p[1].zp_init + size_t(h) * kD + n + j);
-                        }
-                        float o[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) o[k] = dead ? 0.f : fmaf(l, z[k], kPreUnit * __uint_as_float(v[j + k]));
-                        *reinterpret_cast<float4 *>(part + 4 + n + j) = make_float4(o[0], o[1], o[2], o[3]);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 z = *reinterpret_cast<const float4 *>(sh.z0_v() + n + j);
+                        const uint32_t *o = &v[j / 16][j % 16];
+                        const float4 x = make_float4(fmaf(l, z.x, kPreUnit * __uint_as_float(o[0])), fmaf(l, z.y, kPreUnit * __uint_as_float(o[1])),
+                                                     fmaf(l, z.z, kPreUnit * __uint_as_float(o[2])), fmaf(l, z.w, kPreUnit * __uint_as_float(o[3])));
+                        *reinterpret_cast<float4 *>(row + 4 + n + j) = dead ? make_float4(0.f, 0.f, 0.f, 0.f) : x;
                     }
                 }
+                fence_async_shared();
+                if (r < rows) {
+                    bulk_store(part, row, kPartStride * 4);
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                }
             }
-        }
-    } else if (warp == 12) {
-        // ------------------------------------------------------------------------------ S = Q x^T
-        constexpr uint32_t desc = pre_mma_desc(kPreRows, kPreTok, true);
-        int i = 0;
-#pragma unroll 1
-        for (; i < n_tiles; ++i) {
-            const int buf = i & 1;
-            if (!(ok = mbar_wait(&sh.full[0][buf], i / 2 & 1, kStatKWait))) break;
-            if (i >= 2 && !(ok = mbar_wait(&sh.odone[buf], (i / 2 & 1) ^ 1, kStatVWait))) break;   // the weights in S's place are used
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t qd = k_major_desc(&sh.q[0][0][0], kPreRows * 16, 128), xd = mn_major_desc(&sh.x[0][buf][0][0][0], 128, kD * 16);
-#pragma unroll
-                for (int n = 0; n < kD / 16; ++n)
-                    mma_smem(tmem + kColS + kPreTok * buf, qd + 2 * (kPreRows * 16 / 16) * n, xd + 16 * n, desc, n > 0);
-                mma_commit(&sh.sdone[buf]);
-            }
+        } else if (warp == 12) {
+            // -------------------------------------------------------------------------- S = Q x^T
+            constexpr uint32_t desc = pre_mma_desc(kPreRows, kPreTok, true);
+            int i = 0;
+            int issued = min(2, n_tiles);
+            if (elect_one())
+                for (int k = 0; k < issued; ++k) load_tile(0, k);
             __syncwarp();
-        }
-        if (!ok && lane == 0) sh.dead = 1;
-        __syncthreads();
-        if (sh.dead)   // products in flight
-            for (int k = max(i - 2, 0); k < i; ++k) mbar_wait(&sh.sdone[k & 1], k / 2 & 1, kStatDrain);
-    } else {
-        // ------------------------------------------------------------------------------ O += P y
-        constexpr uint32_t desc = pre_mma_desc(kPreRows, kD, false);
-        int i = 0;
+            load_q(threadIdx.x - 256);
 #pragma unroll 1
-        for (; i < n_tiles; ++i) {
-            const int buf = i & 1;
-            if (!(ok = mbar_wait(&sh.full[1][buf], i / 2 & 1, kStatVWait))) break;
-            if (!(ok = mbar_wait(&sh.pfull[buf], i / 2 & 1, kStatVWait))) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t yd = k_major_desc(&sh.x[1][buf][0][0][0], kD * 16, 128);
+            for (; i < n_tiles; ++i) {
+                const int tile = done + i, buf = tile & 1;
+                if (!(ok = mbar_wait(&sh.full[0][buf], tile >> 1 & 1, kStatKWait))) break;
+                if (issued < n_tiles) {
+                    if (elect_one()) load_tile(0, issued);
+                    ++issued;
+                }   // the words of this tile are read
+                __syncwarp();
+                if (tile >= 2 && !(ok = mbar_wait(&sh.odone[buf], (tile >> 1 & 1) ^ 1, kStatVWait))) break;   // the weights in S's place are used
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t qd = k_major_desc(&sh.q[0][0][0], kPreRows * 16, 128), xd = mn_major_desc(&sh.x[0][buf][0][0][0], 128, kD * 16);
 #pragma unroll
-                for (int n = 0; n < kPreTok / 16; ++n)
-                    mma_tmem(tmem + kColO, tmem + kColS + kPreTok * buf + 8 * n, yd + 2 * (kD * 16 / 16) * n, desc, i > 0 || n > 0);
-                mma_commit(&sh.odone[buf]);
+                    for (int n = 0; n < kD / 16; ++n)
+                        mma_smem(tmem + kColS + kPreTok * buf, qd + 2 * kPreRows * n, xd + 16 * n, desc, n > 0);
+                    mma_commit(&sh.sdone[buf]);
+                }
+                __syncwarp();
             }
+            if (!ok && lane == 0) sh.dead = 1;
+            __syncthreads();
+            if (sh.dead) {   // products and copies in flight
+                for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k & 1], k >> 1 & 1, kStatDrain);
+                for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k & 1], k >> 1 & 1, kStatDrain);
+            }
+        } else {
+            // -------------------------------------------------------------------------- O += P y
+            constexpr uint32_t desc = pre_mma_desc(kPreRows, kD, false);
+            int i = 0;
+            int issued = min(2, n_tiles);
+            if (elect_one())
+                for (int k = 0; k < issued; ++k) load_tile(1, k);
             __syncwarp();
+            load_q(threadIdx.x - 256);
+#pragma unroll 1
+            for (; i < n_tiles; ++i) {
+                const int tile = done + i, buf = tile & 1;
+                if (!(ok = mbar_wait(&sh.full[1][buf], tile >> 1 & 1, kStatVWait))) break;
+                if (issued < n_tiles) {
+                    if (elect_one()) load_tile(1, issued);
+                    ++issued;
+                }
+                __syncwarp();
+                if (!(ok = mbar_wait(&sh.pfull[buf], tile >> 1 & 1, kStatVWait))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t yd = k_major_desc(&sh.x[1][buf][0][0][0], kD * 16, 128);
+#pragma unroll
+                    for (int n = 0; n < kPreTok / 16; ++n)
+                        mma_tmem(tmem + kColO, tmem + kColS + kPreTok * buf + 8 * n, yd + 2 * kD * n, desc, i > 0 || n > 0);
+                    mma_commit(&sh.odone[buf]);
+                }
+                __syncwarp();
+            }
+            if (!ok && lane == 0) sh.dead = 1;
+            __syncthreads();
+            if (sh.dead) {
+                for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.odone[k & 1], k >> 1 & 1, kStatDrain);
+                for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k & 1], k >> 1 & 1, kStatDrain);
+            }
         }
-        if (!ok && lane == 0) sh.dead = 1;
+        done += n_tiles;
+        tc_fence_before();
+        fence_async_shared();
         __syncthreads();
-        if (sh.dead)
-            for (int k = max(i - 2, 0); k < i; ++k) mbar_wait(&sh.odone[k & 1], k / 2 & 1, kStatDrain);
+        tc_fence_after();
+        if (sh.dead) break;   // the runs that are left: their parts are marked below
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    if (sh.dead && warp >= 8 && warp < 12) {
+        // every part of this CTA makes the results of its rows NaN (the runs that it did not come to have nothing else to say so)
+        for (long long at = plan.first(blockIdx.x); at < last; at += plan.n_int - at % plan.n_int) {
+            const int unit = int(at / plan.n_int), row = unit % plan.row_tiles * kPreRows + (threadIdx.x & 127), h = unit / plan.row_tiles;
+            if (row >= a.rows) continue;
+            float *part = a.scratch + ((size_t(row / G * a.Hkv + h) * plan.n_parts + blockIdx.x - plan.cta_of((long long)unit * plan.n_int)) * G + row % G) * kPartStride;
+            part[0] = -INFINITY;
+            part[1] = __int_as_float(0x7fc00000);
+        }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the results are where the join finds them
     if (warp == 12) tmem_free(tmem, kColumns);
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the merge waits for this kernel, and with it for the one before
 }
 
 // =========================================================================================
-// The tokens that a sequence has cached itself, from the state behind the prefix, and the new one: one CTA per stream, as the
-// checkpointed step has one per segment.
+// The tokens that a sequence has cached itself, from the state behind the prefix, and the new one: one CTA per stream, as in the fused
+// step of adkv_fused.cu.  Its part comes behind those of the prefix's runs.
+template <int G, int TOK>
+struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
+    float *part;   // [G][kPartStride]
+    __device__ __forceinline__ void store(const VArgs &, int, int, int c0, const float (&acc)[G][4]) const
+    {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float l = this->denominator(g);
+            if (c0 == 0) *reinterpret_cast<float2 *>(part + g * kPartStride) = make_float2(this->m[g], l);
+            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+        }
+    }
+    // a bounded wait gave up, or the length did not fit: the result is NaN
+    __device__ __forceinline__ void give_up(int c0) const
+    {
+#pragma unroll 1
+        for (int g = 0; g < G; ++g) {
+            if (c0 == 0) *reinterpret_cast<float2 *>(part + g * kPartStride) = make_float2(-INFINITY, __int_as_float(0x7fc00000));
+            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+};
+
+// Parts of the prefix's runs that the rows of a sequence have (G divides the rows of a unit: all of its heads lie in one).
+__device__ __forceinline__ int prefix_parts(const PrefixPlan &plan, int b, int h, int G)
+{
+    if (!plan.ctas) return 0;
+    const long long at = (long long)(h * plan.row_tiles + b * G / kPreRows) * plan.n_int;
+    return plan.cta_of(at + plan.n_int - 1) - plan.cta_of(at) + 1;
+}
+
 template <int BITS, int G>
 __global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, const float *__restrict__ k_state, const float *__restrict__ v_state,
-                                                        const int *__restrict__ seq_lens, float scaling, float *__restrict__ scratch, int n_parts)
+                                                        const int *__restrict__ seq_lens, float scaling, float *__restrict__ scratch,
+                                                        const __grid_constant__ PrefixPlan plan)
 {
     constexpr int TOK = 64, ST = 2;
     __shared__ alignas(128) uint8_t kbuf[ST * Tile<BITS, TOK>::BYTES];
@@ -410,31 +530,25 @@ __global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, cons
     const int bh = blockIdx.x, b = bh / ka.Hkv, h = bh % ka.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    float *part = scratch + (size_t(bh) * n_parts + n_parts - 1) * G * kPartStride;
+    bool fits = true;
     if (seq_lens) {
-        const int T = seq_lens[b];
-        if (T < 0 || T / Codec<BITS>::TPW >= ka.n_super_cap) {   // does not fit: nothing is appended, the outputs of the sequence are NaN
-            if (threadIdx.x == 0) atomicExch(&g_status, kStatCapacity);
-            for (int i = threadIdx.x; i < G * kPartStride; i += 64)
-                part[i] = i % kPartStride == 0 ? -INFINITY : i % kPartStride == 1 ? __int_as_float(0x7fc00000) : 0.f;
-            return;
-        }
-        ka.T = T;
-        va.T = T;
+        ka.T = va.T = seq_lens[b];
+        fits = ka.T >= 0 && ka.T / Codec<BITS>::TPW < ka.n_super_cap;
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) { mbar_init(&kbar[i], 1); mbar_init(&vbar[i], 1); }
         fs.init_barriers(1);
         mbar_init_fence();
+        if (!fits) atomicExch(&g_status, kStatCapacity);
     }
     __syncthreads();
     const float *init = (warp == 0 ? k_state : v_state) + size_t(h) * 2 * kD;
     const Seg seg{0, ka.T, true, init, nullptr, 0};
-    if (warp == 0) {
+    if (warp == 0 && fits) {
         RingSink<G, 1, TOK> sink{&fs, 0, 0};
         k_warp<BITS, G, kArithFma, RingSink<G, 1, TOK>, ST, false, BITS == 4 && G == 1, 8, TOK>(ka, seg, b, h, lane, kbuf, kbar, red, sink);
-    } else {
-        using Src = PartialSrc<G, false, TOK>;
+    } else if (warp == 1) {
+        using Src = OwnSrc<G, TOK>;
         Src src;
         src.sh = &fs;
         src.wts = wts;
@@ -442,54 +556,136 @@ __global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, cons
         src.scale2 = scaling * 1.4426950408889634f;
         src.n_tiles = (ka.T + TOK - 1) / TOK;
         src.t_begin = 0;
-        src.part = part;
+        src.part = scratch + (size_t(bh) * plan.n_parts + prefix_parts(plan, b, h, G)) * G * kPartStride;
         src.init();
-        v_warp<BITS, G, kArithFma, Src, ST, false, BITS == 4 && G == 1, TOK>(va, seg, b, h, lane, vbuf, vbar, wts, src);
+        if (fits) v_warp<BITS, G, kArithFma, Src, ST, false, BITS == 4 && G == 1, TOK>(va, seg, b, h, lane, vbuf, vbar, wts, src);
+        else src.give_up(4 * lane);
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // what waits for this kernel waits for the prefix kernel, too
 }
 
-// Intervals of a run: few enough runs to be set up cheaply, enough to fill the chip evenly.  Two CTAs share an SM.
-static int run_intervals(int tokens, int interval, int Hkv, int row_tiles)
+// out[b, hq] = sum_j x_j 2^(m_j - M) / sum_j l_j 2^(m_j - M) over the parts of a row.  Four warps share a row's parts, a part's 128 sums are
+// 16 bytes a lane; all loads of a row are in flight at once, which is what bounds it.
+constexpr int kJoinWarps = 4, kJoinLoads = 4;
+__global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const float *__restrict__ scratch, __half *__restrict__ out, int Hq, int Hkv,
+                                                                      const __grid_constant__ PrefixPlan plan)
 {
-    if (interval <= 0 || tokens <= interval) return 1;
-    const int n = (tokens + interval - 1) / interval;
-    int best = 1;
-    double least = 1e30;
-    for (int k = 1; k <= n; ++k) {
-        const int runs = (n + k - 1) / k;
-        if (runs > 128) continue;
-        const long long ctas = (long long)runs * Hkv * row_tiles, rounds = (ctas + 2 * kSMs - 1) / (2 * kSMs);
-        const double cost = double(rounds) * (double(k) * interval + 96);
-        if (cost < least) {
-            least = cost;
-            best = k;
+    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float2 ml[kJoinWarps];
+    const int b = blockIdx.x / Hq, hq = blockIdx.x % Hq, G = Hq / Hkv, h = hq / G, g = hq % G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = prefix_parts(plan, b, h, G) + 1;
+    const float *base = scratch + (size_t(b * Hkv + h) * plan.n_parts * G + g) * kPartStride;
+    const size_t stride = size_t(G) * kPartStride;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int j0 = warp; j0 < n; j0 += kJoinWarps * kJoinLoads) {
+        float2 part_ml[kJoinLoads];
+        float4 x[kJoinLoads];
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) {
+            const float *part = base + size_t(min(j0 + u * kJoinWarps, n - 1)) * stride;
+            part_ml[u] = *reinterpret_cast<const float2 *>(part);
+            x[u] = *reinterpret_cast<const float4 *>(part + 4 + 4 * lane);
         }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u) top = fmaxf(top, part_ml[u].x);
+        const float corr = m == -INFINITY ? 0.f : exp2f(m - top);
+        l *= corr;
+        o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr;
+#pragma unroll
+        for (int u = 0; u < kJoinLoads; ++u)
+            if (j0 + u * kJoinWarps < n) {
+                const float w = part_ml[u].x == -INFINITY ? 0.f : exp2f(part_ml[u].x - top);
+                l = fmaf(part_ml[u].y, w, l);   // a NaN: the part could not be finished
+                o.x = fmaf(x[u].x, w, o.x);
+                o.y = fmaf(x[u].y, w, o.y);
+                o.z = fmaf(x[u].z, w, o.z);
+                o.w = fmaf(x[u].w, w, o.w);
+            }
+        m = top;
     }
-    return best;
+    sums[warp][lane] = o;
+    if (lane == 0) ml[warp] = make_float2(m, l);
+    __syncthreads();
+    const int c = threadIdx.x;
+    float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) M = fmaxf(M, ml[w].x);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = ml[w].x == -INFINITY ? 0.f : exp2f(ml[w].x - M);
+        L = fmaf(ml[w].y, f, L);
+        A = fmaf(reinterpret_cast<const float *>(&sums[w][0])[c], f, A);
+    }
+    out[size_t(blockIdx.x) * kD + c] = __float2half_rn(A / L);
 }
-static int prefix_runs(int tokens, int interval, int Hkv, int row_tiles, int *run)
+
+// A CTA for each of the 296 places (two share an SM), but no fewer than 128 tokens to one: setting up a run and storing its result costs
+// about as much as that many.
+static PrefixPlan prefix_plan(int tokens, int interval, int B, int G, int Hkv)
 {
-    if (tokens == 0) { *run = 0; return 0; }
-    *run = interval > 0 ? run_intervals(tokens, interval, Hkv, row_tiles) * interval : tokens;
-    return (tokens + *run - 1) / *run;
+    PrefixPlan p{};
+    p.row_tiles = int(((long long)B * G + kPreRows - 1) / kPreRows);
+    p.n_parts = 1;   // the sequence's own
+    if (tokens == 0 || B == 0) return p;
+    p.interval = interval > 0 ? interval : tokens;
+    p.n_int = int(((long long)tokens + p.interval - 1) / p.interval);
+    p.n = (long long)p.n_int * Hkv * p.row_tiles;
+    const int least = (128 + p.interval - 1) / p.interval;
+    p.ctas = int(std::min((long long)2 * kSMs, (p.n + least - 1) / least));
+    p.n_parts += int((long long)(p.n_int - 1) * p.ctas / p.n) + 2;
+    return p;
 }
 
 }  // namespace adkv
 
 using namespace adkv;
 
-ADKV_HIDDEN int adkv_launch_merge(const float *scratch, __half *out, int B, int Hq, int Hkv, int n_seg, cudaStream_t s);
-
 ADKV_DEFINE_TU_STATUS(adkv_tu_status_prefix)
 
 template <int BITS>
-static int launch_prefix(const PrefixArgs &a, cudaStream_t s)
+static int launch_prefix(const PrefixArgs &a, const PrefixPlan &plan, cudaStream_t s)
 {
-    constexpr int bytes = int(sizeof(PrefixShared));
+    constexpr int bytes = int(sizeof(PrefixShared<BITS>));
     static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
     const auto kernel = prefix_kernel<BITS>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return launch_status();
-    kernel<<<a.n_runs * a.Hkv * a.row_tiles, kPreThreads, bytes, s>>>(a);
+    kernel<<<plan.ctas, kPreThreads, bytes, s>>>(a, plan);
+    return launch_status();
+}
+
+// As a programmatic dependent of the launch before it, or, where that is refused, behind it: by then something has run that must not be
+// left without its end.
+template <class... Params, class... Args>
+static int launch_beside(void (*kernel)(Params...), int grid, int block, cudaStream_t s, const Args &...args)
+{
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+        cudaGetLastError();
+        kernel<<<grid, block, 0, s>>>(args...);
+    }
+    return launch_status();
+}
+
+template <int BITS, int G>
+static int launch_own(const KArgs &ka, const VArgs &va, const float *k_state, const float *v_state, const int *seq_lens, float scaling,
+                      float *scratch, const PrefixPlan &plan, int B, cudaStream_t s)
+{
+    const auto kernel = prefix_own_kernel<BITS, G>;
+    if (plan.ctas) return launch_beside(kernel, B * ka.Hkv, 64, s, ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
+    kernel<<<B * ka.Hkv, 64, 0, s>>>(ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
     return launch_status();
 }
 
@@ -498,9 +694,8 @@ extern "C" {
 long long adkv_decode_attn_prefix_scratch_bytes(int B, int Hq, int Hkv, int prefix_tokens, int interval)
 {
     if (B < 0 || Hq <= 0 || Hkv <= 0 || prefix_tokens < 0 || interval < 0 || Hq % Hkv != 0) return ADKV_E_SHAPE;
-    int run;
-    const int runs = prefix_runs(prefix_tokens, interval, Hkv, int(((long long)B * (Hq / Hkv) + kPreRows - 1) / kPreRows), &run);
-    return (long long)B * Hq * (runs + 1) * kPartStride * (long long)sizeof(float);
+    const PrefixPlan plan = prefix_plan(prefix_tokens, interval, B, Hq / Hkv, Hkv);
+    return (long long)B * Hq * plan.n_parts * kPartStride * (long long)sizeof(float);
 }
 
 int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
@@ -508,7 +703,7 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
                             void *scratch, long long scratch_bytes, int B, int Hq, int Hkv, int D, int n_super_cap, int bits, float scaling,
                             float scale_min, float scale_max, unsigned flags, void *stream)
 {
-    if (!q || !prefix || !k_cache || !v_cache || !k_new || !v_new || !out || !params_ok(kp) || !params_ok(vp) || !k_tail || !v_tail || !scratch ||
+    if (!q || !prefix || !k_cache || !v_cache || !k_new || !v_new || !out || !params_ok(kp) || !params_ok(vp) || !k_tail || !v_tail ||
         !prefix->k_tail || !prefix->v_tail || (prefix->tokens > 0 && (!prefix->k_cache || !prefix->v_cache)))
         return ADKV_E_NULL;
     if (D != kD) return ADKV_E_HEAD_DIM;
@@ -531,7 +726,9 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
         return ADKV_E_ALIGN;
     const long long rows = (long long)B * G;
     if (rows > (1 << 24)) return ADKV_E_SHAPE;
-    if (scratch_bytes < adkv_decode_attn_prefix_scratch_bytes(B, Hq, Hkv, P, iv)) return ADKV_E_SCRATCH;
+    const long long need = adkv_decode_attn_prefix_scratch_bytes(B, Hq, Hkv, P, iv);
+    if (need > 0 && !scratch) return ADKV_E_NULL;
+    if (scratch_bytes < need) return ADKV_E_SCRATCH;
     if (B == 0) return 0;
 
     PrefixArgs pa{};
@@ -546,13 +743,9 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     pa.Hq = Hq;
     pa.Hkv = Hkv;
     pa.rows = int(rows);
-    pa.row_tiles = (pa.rows + kPreRows - 1) / kPreRows;
     pa.n_super_cap = prefix->n_super_cap;
     pa.n_ckpt_cap = prefix->n_ckpt_cap;
     pa.tokens = P;
-    pa.interval = iv;
-    pa.n_runs = prefix_runs(P, iv, Hkv, pa.row_tiles, &pa.run);
-    pa.n_parts = pa.n_runs + 1;
     pa.scaling = scaling;
     pa.smin = scale_min;
     pa.smax = scale_max;
@@ -562,13 +755,14 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     const VArgs va{static_cast<uint8_t *>(v_cache), static_cast<const __half *>(v_new), static_cast<__half *>(out), pa.p[1], Hq, Hkv, T, n_super_cap,
                    scale_min, scale_max, D, static_cast<float *>(v_tail), keep};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (pa.n_runs)
-        if (int rc = bits == 4 ? launch_prefix<4>(pa, s) : launch_prefix<2>(pa, s)) return rc;
-    ADKV_DISPATCH_H(bits, G, (prefix_own_kernel<BITS, G><<<B * Hkv, 64, 0, s>>>(ka, va, static_cast<const float *>(prefix->k_tail),
-                                                                               static_cast<const float *>(prefix->v_tail),
-                                                                               static_cast<const int *>(seq_lens), scaling, pa.scratch, pa.n_parts)))
-    if (int rc = launch_status()) return rc;
-    return adkv_launch_merge(pa.scratch, static_cast<__half *>(out), B, Hq, Hkv, pa.n_parts, s);
+    const PrefixPlan plan = prefix_plan(P, iv, B, G, Hkv);
+    if (plan.ctas)
+        if (int rc = bits == 4 ? launch_prefix<4>(pa, plan, s) : launch_prefix<2>(pa, plan, s)) return rc;
+    int rc = 0;
+    ADKV_DISPATCH_H(bits, G, (rc = launch_own<BITS, G>(ka, va, static_cast<const float *>(prefix->k_tail), static_cast<const float *>(prefix->v_tail),
+                                                         static_cast<const int *>(seq_lens), scaling, pa.scratch, plan, B, s)))
+    if (rc) return rc;
+    return launch_beside(prefix_join_kernel, B * Hq, 32 * kJoinWarps, s, pa.scratch, static_cast<__half *>(out), Hq, Hkv, plan);
 }
 
 }  // extern "C"

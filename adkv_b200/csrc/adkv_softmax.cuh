@@ -158,39 +158,6 @@ struct SoftmaxSrc {
 
 constexpr int kPartStride = 4 + kD;   // floats per (stream, segment, head): max (log2 units), denominator, 2 pad, kD sums
 
-// Source that leaves maximum, denominator and sums of a segment instead of a result.
-template <int G, bool HALF_W, int TOK>
-struct PartialSrc : SoftmaxSrc<G, 1, HALF_W, TOK> {
-    float *part;   // [G][kPartStride] of this (stream, segment)
-    __device__ __forceinline__ void store(const VArgs &, int, int, int c0, const float (&acc)[G][4]) const
-    {
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float l = this->denominator(g);
-            if (c0 == 0) {
-                part[g * kPartStride] = this->m[g];
-                part[g * kPartStride + 1] = l;
-            }
-            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) =
-                make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
-        }
-    }
-    // The segment could not be finished (a bounded wait gave up; the status word says which): leave a partial
-    // that turns the merged output of these heads into NaN, so that neither the scratch contents of an earlier
-    // call nor an output that silently lacks a segment can pass for a result.
-    __device__ __forceinline__ void give_up(int c0) const
-    {
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if (c0 == 0) {
-                part[g * kPartStride] = -INFINITY;
-                part[g * kPartStride + 1] = __int_as_float(0x7fc00000);
-            }
-            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    }
-};
-
 struct CkptArgs {
     float *k_ckpt, *v_ckpt;   // [B*Hkv][n_ckpt_cap][2][kD]; entry k = state before token (k+1)*interval
     int interval, n_ckpt_cap;

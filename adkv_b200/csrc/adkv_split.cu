@@ -22,6 +22,38 @@ namespace adkv {
 template <int TOK>
 constexpr int kSplitStages = TOK == 64 ? 2 : 3;
 
+template <int G, bool HALF_W, int TOK>
+struct PartialSrc : SoftmaxSrc<G, 1, HALF_W, TOK> {
+    float *part;   // [G][kPartStride] of this (stream, segment)
+    __device__ __forceinline__ void store(const VArgs &, int, int, int c0, const float (&acc)[G][4]) const
+    {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float l = this->denominator(g);
+            if (c0 == 0) {
+                part[g * kPartStride] = this->m[g];
+                part[g * kPartStride + 1] = l;
+            }
+            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) =
+                make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+        }
+    }
+    // The segment could not be finished (a bounded wait gave up; the status word says which): leave a partial
+    // that turns the merged output of these heads into NaN, so that neither the scratch contents of an earlier
+    // call nor an output that silently lacks a segment can pass for a result.
+    __device__ __forceinline__ void give_up(int c0) const
+    {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (c0 == 0) {
+                part[g * kPartStride] = -INFINITY;
+                part[g * kPartStride + 1] = __int_as_float(0x7fc00000);
+            }
+            *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+};
+
 // Guarded chunk bodies as function calls (see k_chunk_guarded): measured 2-3 % faster for 4-bit codes with one query
 // head per KV head at every batch and checkpoint interval tried; not measured for the other instantiations.
 template <int BITS, int G>
@@ -169,7 +201,7 @@ ADKV_DEFINE_TU_STATUS(adkv_tu_status_split)
 
 // The merge follows the segment kernel on the same stream as its programmatic dependent: set up early, started
 // when the segment kernel is done (griddepcontrol.wait in the kernel orders the memory).
-ADKV_HIDDEN int adkv_launch_merge(const float *scratch, __half *out, int B, int Hq, int Hkv, int n_seg, cudaStream_t s)
+static int launch_merge(const float *scratch, __half *out, int B, int Hq, int Hkv, int n_seg, cudaStream_t s)
 {
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -251,7 +283,7 @@ int adkv_decode_attn_ckpt(const void *q, void *k_cache, void *v_cache, const voi
                           static_cast<float *>(scratch))))
     }
     if (int rc = launch_status()) return rc;
-    return adkv_launch_merge(static_cast<const float *>(scratch), static_cast<__half *>(out), B, Hq, Hkv, n_seg, s);
+    return launch_merge(static_cast<const float *>(scratch), static_cast<__half *>(out), B, Hq, Hkv, n_seg, s);
 }
 
 }  // extern "C"
