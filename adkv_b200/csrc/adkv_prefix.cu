@@ -17,6 +17,7 @@
 #include "adkv_host.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "adkv_softmax.cuh"
 #include "adkv_tensor.cuh"
@@ -42,10 +43,14 @@ struct PrefixArgs {
 // How the prefix is laid over CTAs.  The intervals of all units (128 rows of one head) form one line, of which every CTA takes an equal
 // piece: whole intervals, so that it can enter anywhere.  A piece that crosses from one unit to the next is two runs.
 struct PrefixPlan {
-    int n_int, interval, row_tiles, ctas, n_parts;   // intervals of a unit, their tokens; n_parts: room for the runs of a unit
+    int n_int, interval, row_tiles, ctas, n_parts;   // intervals of a unit, their tokens; n_parts: room for the parts of a stream
+    int each;                                        // CTAs of a unit where no piece crosses from one to the next, else 0
     long long n;                                     // intervals of all units
     __host__ __device__ long long first(int cta) const { return n * cta / ctas; }
     __host__ __device__ int cta_of(long long at) const { return int(((at + 1) * ctas - 1) / n); }
+    // first CTA of a unit, and how many have a piece of it
+    __host__ __device__ int first_cta(int unit) const { return each ? unit * each : cta_of((long long)unit * n_int); }
+    __host__ __device__ int parts(int unit) const { return each ? each : cta_of((long long)unit * n_int + n_int - 1) - first_cta(unit) + 1; }
 };
 
 template <int BITS>
@@ -53,7 +58,7 @@ struct PrefixShared {
     alignas(128) __half q[kD / 8][kPreRows][8];          // [channel / 8][row][channel % 8]
     alignas(128) __half x[2][2][kPreTok / 8][kD][8];     // K, V; buffer; [token / 8][channel][token % 8]
     alignas(128) uint32_t words[2][2][kPreTok * BITS / 32][kD];   // packed tiles of K and V
-    float z0[kD];                                        // zero points of K before the run
+    alignas(16) float z0[kD];                            // zero points of K before the run
     // The results of the run lie in x and what follows, a row every kPartStride floats (no two of eight in the same banks), and the zero
     // points of V before the run in the last row of words, where only their own thread has read.
     __device__ float *row(int r) { return reinterpret_cast<float *>(&x[0][0][0][0][0]) + r * kPartStride; }
@@ -82,15 +87,23 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 struct PrefixChan {
     float zp, s, alpha, beta, tc;
 };
-// Eight tokens, fields 0..7 of w, contracted as in k_chunk2; the values go to dst.
+// Eight tokens, fields 0..7 of w, contracted as in k_chunk2; the values go to dst.  GUARDED: with the eps guard, the clamps and the
+// end of the run (left tokens).  Otherwise least and most take in the scale before every fourth token, which tells afterwards whether
+// the guards would have done anything.
 template <int BITS, bool GUARDED>
-__device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS> &fc, PrefixChan &c, float smin, float smax, float eps, int left, uint8_t *dst)
+__device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS> &fc, PrefixChan &c, float smin, float smax, int left, float &least,
+                                              float &most, uint8_t *dst)
 {
-    float x[8];
+    float x[8], s0 = 0.f;
     static_for<8>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
+        if (!GUARDED && j == 0) s0 = c.s;
+        if (!GUARDED && j == 4) {
+            least = fminf(fminf(least, s0), c.s);
+            most = fmaxf(fmaxf(most, s0), c.s);
+        }
         const float q = fc.template code<j % 4>(j < 4 ? w : w >> (4 * BITS));
-        const float rh = __fmul_rn(q, GUARDED ? fmaxf(c.s, eps) : c.s);
+        const float rh = __fmul_rn(q, GUARDED ? fmaxf(c.s, kEps / kPreUnit) : c.s);
         x[j] = __fadd_rn(rh, c.zp);
         if (GUARDED && j >= left) x[j] = 0.f;   // behind the last token: whatever the words hold there does not count
         c.zp = fmaf(c.alpha, rh, c.zp);
@@ -98,15 +111,6 @@ __device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS
         if (GUARDED) c.s = fminf(fmaxf(c.s, smin), smax);
     });
     *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
-}
-// The guarded and the ragged window, by a call that keeps them out of the loop and of its registers.
-template <int BITS>
-__device__ __noinline__ float2 prefix_window_guarded(uint32_t w, PrefixChan c, float smin, float smax, int left, uint8_t *dst)
-{
-    FieldConsts<BITS> fc;
-    fc.init();
-    prefix_window<BITS, true>(w, fc, c, smin * (1.f / kPreUnit), smax * (1.f / kPreUnit), kEps * (1.f / kPreUnit), left, dst);
-    return make_float2(c.zp, c.s);
 }
 
 __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreSlack
@@ -125,6 +129,21 @@ __device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t 
 {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)), "r"(smem_u32(src)), "r"(bytes) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// The 64 columns of a tile, 16 at a time: the next ones are on their way while use() works on these.
+template <class F>
+__device__ __forceinline__ void for_columns(uint32_t cols, const F &use)
+{
+    uint32_t v[2][16];
+    tmem_ld(v[0], cols);
+    tmem_wait_ld(v[0]);
+#pragma unroll
+    for (int n = 0; n < kPreTok / 16; ++n) {
+        if (n + 1 < kPreTok / 16) tmem_ld(v[(n + 1) & 1], cols + 16 * (n + 1));
+        use(16 * n, v[n & 1]);
+        if (n + 1 < kPreTok / 16) tmem_wait_ld(v[(n + 1) & 1]);
+    }
 }
 
 template <int BITS>
@@ -226,13 +245,15 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                 start = __half2float(p.zp_init[po]);
                 s = __half2float(p.scale_init[po]);
             }
-            SafeRange safe{0.f, INFINITY};
-            const float be[1] = {beta}, tg[1] = {target};
-            safe.template init<BITS, 1>(be, tg, a.smin, a.smax);
-            const float lo = safe.lo * (1.f / kPreUnit), hi = safe.hi * (1.f / kPreUnit);   // scales that eight updates cannot bring to a bound
+            // Scales from which four updates cannot leave the bounds: inside, guards and clamps are the identity.  (SafeRange is the
+            // same for eight; of 4-bit caches with the usual parameters 2 % of the windows begin outside that, next to none outside this.)
+            const float g0 = 1.f - beta * target, g1 = g0 + beta * float(Codec<BITS>::BIAS), gmn = fminf(fminf(g0, g1), 1.f), gmx = fmaxf(fmaxf(g0, g1), 1.f);
+            const float lo = gmn > 0.f ? fmaxf(a.smin, kEps) * (1.f / kPreUnit) / (gmn * gmn * gmn * gmn * (1.f - 2e-5f)) : INFINITY;
+            const float hi = a.smax * (1.f / kPreUnit) / (gmx * gmx * gmx * gmx * (1.f + 2e-5f));
             PrefixChan ch{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f)};
             if (which == 0) sh.z0[c] = start;
             uint64_t *freed = which ? sh.odone : sh.sdone;
+            bool tame = true;   // no scale of the warp was outside its interval when last looked at
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i) {
                 const int tile = done + i, buf = tile & 1;
@@ -241,23 +262,43 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                 const uint32_t *row = &sh.words[which][buf][0][c];
                 uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][buf][0][c][0]);
                 int left = ntok - i * kPreTok;
+                // Rounds of 32 tokens without guards first, which is right if every fourth scale was inside its interval: one vote a
+                // round.  Where it was not the round is done again with guards, and so are the next ones at once until it is.
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half, left -= kPreTok / 2) {
+                for (int half = 0; half < 2; ++half, left -= kPreTok / 2, dst += (kPreTok / 16) * kD * 16) {
                     uint32_t w[WORDS / 2];
 #pragma unroll
                     for (int k = 0; k < WORDS / 2; ++k, row += kD) w[k] = *row;
-                    static_for<kPreTok / 16>([&](auto nc) {
-                        constexpr int n = decltype(nc)::value;
-                        const uint32_t word = BITS == 4 ? w[n % (WORDS / 2)] : w[n / 2 % (WORDS / 2)] >> (16 * (n & 1));
-                        if (__all_sync(kFull, ch.s >= lo && ch.s <= hi) && left >= 8 * n + 8) {
-                            prefix_window<BITS, false>(word, fc, ch, 0.f, 0.f, 0.f, 0, dst);
-                        } else {
-                            const float2 state = prefix_window_guarded<BITS>(word, ch, a.smin, a.smax, left - 8 * n, dst);
-                            ch.zp = state.x;
-                            ch.s = state.y;
+                    const float zp = ch.zp, s = ch.s;
+                    bool inside = tame && left >= kPreTok / 2;
+                    if (inside) {
+                        float least = INFINITY, most = -INFINITY;
+                        static_for<kPreTok / 16>([&](auto nc) {
+                            constexpr int n = decltype(nc)::value;
+                            prefix_window<BITS, false>(BITS == 4 ? w[n % (WORDS / 2)] : w[n / 2 % (WORDS / 2)] >> (16 * (n & 1)), fc, ch, 0.f, 0.f, 0, least,
+                                                       most, dst + n * kD * 16);
+                        });
+                        inside = __all_sync(kFull, least >= lo && most <= hi);
+                    }
+                    if (!inside) {
+                        ch.zp = zp;
+                        ch.s = s;
+                        float least = INFINITY, most = -INFINITY;
+#pragma unroll 1
+                        for (int n = 0; n < kPreTok / 16; ++n) {   // rolled: the words move up
+                            least = fminf(least, ch.s);
+                            most = fmaxf(most, ch.s);
+                            prefix_window<BITS, true>(w[0], fc, ch, a.smin * (1.f / kPreUnit), a.smax * (1.f / kPreUnit), left - 8 * n, least, most,
+                                                      dst + n * kD * 16);
+                            if (BITS == 2 && !(n & 1)) {
+                                w[0] >>= 16;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k + 1 < WORDS / 2; ++k) w[k] = w[k + 1];
+                            }
                         }
-                        dst += kD * 16;
-                    });
+                        tame = __all_sync(kFull, least >= lo && most <= hi);
+                    }
                 }
                 fence_async_shared();
                 warp_arrive(&sh.full[which][buf], lane);
@@ -270,76 +311,74 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             const int e = warp & 3, r = 32 * e + lane;
             const bool busy = 32 * e < rows;
             const uint32_t lanes = tmem + (uint32_t(32 * e) << 16);
-            const float f = fmaxf(fabsf(scale2) * kPreUnit, 1e-30f);   // not 0: masked columns are -inf times this
+            const float f = fabsf(scale2) * kPreUnit;
             const int idle = e == 0 ? 4 - (rows + 31) / 32 : 0;        // warps without rows do not take part; the first arrives for them
-            float m = -INFINITY, l = 0.f, base = 0.f;
+            float m = -INFINITY, l = 0.f;
             load_q(threadIdx.x - 256);
 #pragma unroll 1
             for (int i = 0; i < n_tiles && busy; ++i) {
                 const int tile = done + i, buf = tile & 1;
                 if (!(ok = mbar_wait(&sh.sdone[buf], tile >> 1 & 1, kStatLFullWait))) break;
-                {
-                    tc_fence_after();
-                    const uint32_t cols = lanes + kColS + kPreTok * buf;
-                    const int left = ntok - i * kPreTok;
-                    uint32_t p[kPreTok / 2];
-                    float top, sum;
-                    // weights with the maximum so far, and the largest column; all columns are read before the first weight is written
-                    const auto weigh = [&](auto whole) {
-                        top = -INFINITY;
-                        sum = 0.f;
+                tc_fence_after();
+                const uint32_t cols = lanes + kColS + kPreTok * buf;
+                const int left = ntok - i * kPreTok;
+                float top = -INFINITY;
+                const auto largest = [&](auto whole) {
+                    for_columns(cols, [&](int n, const uint32_t (&v)[16]) {
 #pragma unroll
-                        for (int n = 0; n < kPreTok; n += 16) {
+                        for (int j = 0; j < 16; j += 2) {
+                            const float s0 = __uint_as_float(v[j]), s1 = __uint_as_float(v[j + 1]);
+                            if (decltype(whole)::value) top = fmaxf(fmaxf(top, s0), s1);
+                            else top = fmaxf(fmaxf(top, n + j < left ? s0 : -INFINITY), n + j + 1 < left ? s1 : -INFINITY);
+                        }
+                    });
+                };
+                if (left >= kPreTok) largest(std::true_type{});
+                else largest(std::false_type{});
+                top *= f;
+                const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
+                if (__any_sync(kFull, grown)) {
+                    const float corr = grown ? exp2_fast(m - top) : 1.f;
+                    if (i > 0) {
+                        // all sums so far are in: O can be changed
+                        if (!(ok = mbar_wait(&sh.odone[buf ^ 1], (tile - 1) >> 1 & 1, kStatVWait))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int n = 0; n < kD; n += 16) {
                             uint32_t v[16];
-                            tmem_ld(v, cols + n);
+                            tmem_ld(v, lanes + kColO + n);
                             tmem_wait_ld(v);
 #pragma unroll
-                            for (int j = 0; j < 16; j += 2) {
-                                float s0 = __uint_as_float(v[j]), s1 = __uint_as_float(v[j + 1]);
-                                if (!decltype(whole)::value) {
-                                    s0 = n + j < left ? s0 : -INFINITY;
-                                    s1 = n + j + 1 < left ? s1 : -INFINITY;
-                                }
-                                top = fmaxf(fmaxf(top, s0), s1);
-                                const float p0 = exp2_fast(fmaf(s0, f, -m)), p1 = exp2_fast(fmaf(s1, f, -m));
-                                sum += p0 + p1;
-                                p[(n + j) / 2] = pack2(p0, p1);
-                            }
-                        }
-                        top *= f;
-                    };
-#pragma unroll 1
-                    for (;;) {
-                        if (left >= kPreTok) weigh(std::true_type{});
-                        else weigh(std::false_type{});
-                        const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
-                        if (!__any_sync(kFull, grown)) break;
-                        const float corr = grown ? exp2_fast(m - top) : 1.f;
-                        if (i > 0) {
-                            // all sums so far are in: O can be changed
-                            if (!(ok = mbar_wait(&sh.odone[buf ^ 1], (tile - 1) >> 1 & 1, kStatVWait))) break;
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int n = 0; n < kD; n += 16) {
-                                uint32_t v[16];
-                                tmem_ld(v, lanes + kColO + n);
-                                tmem_wait_ld(v);
+                            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
-#pragma unroll
-                                for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
-                            }
+                            for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
                         }
-                        l *= corr;
-                        if (grown) m = top;
                     }
-                    if (!ok) break;
-                    l += sum;
-#pragma unroll
-                    for (int j = 0; j < kPreTok / 2; j += 4) tmem_st4(cols + j, p[j], p[j + 1], p[j + 2], p[j + 3]);
-                    tmem_wait_st();
-                    tc_fence_before();
+                    l *= corr;
+                    if (grown) m = top;
                 }
+                // the weights take the place of columns that have been read
+                const auto weigh = [&](auto whole) {
+                    for_columns(cols, [&](int n, const uint32_t (&v)[16]) {
+                        uint32_t p[8];
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float p0 = exp2_fast(fmaf(__uint_as_float(v[j]), f, -m)), p1 = exp2_fast(fmaf(__uint_as_float(v[j + 1]), f, -m));
+                            if (!decltype(whole)::value) {
+                                p0 = n + j < left ? p0 : 0.f;
+                                p1 = n + j + 1 < left ? p1 : 0.f;
+                            }
+                            l += p0 + p1;
+                            p[j / 2] = pack2(p0, p1);
+                        }
+                        tmem_st4(cols + n / 2, p[0], p[1], p[2], p[3]);
+                        tmem_st4(cols + n / 2 + 4, p[4], p[5], p[6], p[7]);
+                    });
+                };
+                if (left >= kPreTok) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                tmem_wait_st();
+                tc_fence_before();
                 warp_arrive(&sh.pfull[buf], lane, 1 + idle);
             }
             const int end = done + n_tiles - 1;
@@ -350,20 +389,25 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             if (busy) {
                 tc_fence_after();
                 const int n_row = rt * kPreRows + r;
-                const int slot = blockIdx.x - plan.cta_of((long long)unit * plan.n_int);
+                const int slot = blockIdx.x - plan.first_cta(unit);
                 float *part = a.scratch + ((size_t(n_row >> log_g) * a.Hkv + h) * plan.n_parts + slot) * (kPartStride << log_g) + (n_row & (G - 1)) * kPartStride;
                 float *row = sh.row(r);
                 // what the zero points before the run add to every logit of the row
-#pragma unroll 4
+                float sum[8] = {};
+#pragma unroll 2
                 for (int k = 0; k < kD / 8; ++k) {
-                    float qv[4];
-                    load_half4(qv, &sh.q[k][r][0]);
+                    const uint4 q8 = *reinterpret_cast<const uint4 *>(&sh.q[k][r][0]);
+                    const float4 z0 = *reinterpret_cast<const float4 *>(&sh.z0[8 * k]), z1 = *reinterpret_cast<const float4 *>(&sh.z0[8 * k + 4]);
+                    const float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
+                    const uint32_t q2[4] = {q8.x, q8.y, q8.z, q8.w};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + j], base);
-                    load_half4(qv, &sh.q[k][r][4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) base = fmaf(qv[j], sh.z0[8 * k + 4 + j], base);
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 qf = __half22float2(*reinterpret_cast<const __half2 *>(&q2[j]));
+                        sum[2 * j] = fmaf(qf.x, z[2 * j], sum[2 * j]);
+                        sum[2 * j + 1] = fmaf(qf.y, z[2 * j + 1], sum[2 * j + 1]);
+                    }
                 }
+                const float base = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
                 *reinterpret_cast<float4 *>(row) = dead ? make_float4(-INFINITY, __int_as_float(0x7fc00000), 0.f, 0.f)
                                                         : make_float4(fmaf(base, fabsf(scale2), m), l, 0.f, 0.f);
 #pragma unroll 1
@@ -471,12 +515,11 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         for (long long at = plan.first(blockIdx.x); at < last; at += plan.n_int - at % plan.n_int) {
             const int unit = int(at / plan.n_int), row = unit % plan.row_tiles * kPreRows + (threadIdx.x & 127), h = unit / plan.row_tiles;
             if (row >= a.rows) continue;
-            float *part = a.scratch + ((size_t(row / G * a.Hkv + h) * plan.n_parts + blockIdx.x - plan.cta_of((long long)unit * plan.n_int)) * G + row % G) * kPartStride;
+            float *part = a.scratch + ((size_t(row / G * a.Hkv + h) * plan.n_parts + blockIdx.x - plan.first_cta(unit)) * G + row % G) * kPartStride;
             part[0] = -INFINITY;
             part[1] = __int_as_float(0x7fc00000);
         }
     }
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the results are where the join finds them
     if (warp == 12) tmem_free(tmem, kColumns);
 }
 
@@ -510,16 +553,15 @@ struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
 __device__ __forceinline__ int prefix_parts(const PrefixPlan &plan, int b, int h, int G)
 {
     if (!plan.ctas) return 0;
-    const long long at = (long long)(h * plan.row_tiles + b * G / kPreRows) * plan.n_int;
-    return plan.cta_of(at + plan.n_int - 1) - plan.cta_of(at) + 1;
+    return plan.parts(h * plan.row_tiles + b * G / kPreRows);
 }
 
-template <int BITS, int G>
+template <int BITS, int G, int TOK>
 __global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, const float *__restrict__ k_state, const float *__restrict__ v_state,
                                                         const int *__restrict__ seq_lens, float scaling, float *__restrict__ scratch,
                                                         const __grid_constant__ PrefixPlan plan)
 {
-    constexpr int TOK = 64, ST = 2;
+    constexpr int ST = TOK == 64 ? 2 : 3;   // tiles in flight
     __shared__ alignas(128) uint8_t kbuf[ST * Tile<BITS, TOK>::BYTES];
     __shared__ alignas(128) uint8_t vbuf[ST * Tile<BITS, TOK>::BYTES];
     __shared__ alignas(16) float red[G * 8 * kRedRow];
@@ -624,8 +666,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const floa
     out[size_t(blockIdx.x) * kD + c] = __float2half_rn(A / L);
 }
 
-// A CTA for each of the 296 places (two share an SM), but no fewer than 128 tokens to one: setting up a run and storing its result costs
-// about as much as that many.
+// Two CTAs share an SM, 296 places.  A run costs, besides its tokens, what filling and emptying the pipeline and storing the result take, about
+// as long as 300 tokens: so either every unit gets the same number of CTAs, or the line is cut evenly and most CTAs come to have two runs.
 static PrefixPlan prefix_plan(int tokens, int interval, int B, int G, int Hkv)
 {
     PrefixPlan p{};
@@ -635,9 +677,11 @@ static PrefixPlan prefix_plan(int tokens, int interval, int B, int G, int Hkv)
     p.interval = interval > 0 ? interval : tokens;
     p.n_int = int(((long long)tokens + p.interval - 1) / p.interval);
     p.n = (long long)p.n_int * Hkv * p.row_tiles;
-    const int least = (128 + p.interval - 1) / p.interval;
-    p.ctas = int(std::min((long long)2 * kSMs, (p.n + least - 1) / least));
-    p.n_parts += int((long long)(p.n_int - 1) * p.ctas / p.n) + 2;
+    const int units = Hkv * p.row_tiles, each = std::min(2 * kSMs / units, p.n_int), places = 2 * kSMs;
+    const long long even = (p.n + places - 1) / places, whole = each ? (p.n_int + each - 1) / each : even;
+    p.each = whole * p.interval <= even * p.interval + 300 ? each : 0;
+    p.ctas = p.each ? units * each : int(std::min((long long)places, p.n));
+    p.n_parts += p.each ? p.each : int((long long)(p.n_int - 1) * p.ctas / p.n) + 2;
     return p;
 }
 
@@ -683,7 +727,7 @@ template <int BITS, int G>
 static int launch_own(const KArgs &ka, const VArgs &va, const float *k_state, const float *v_state, const int *seq_lens, float scaling,
                       float *scratch, const PrefixPlan &plan, int B, cudaStream_t s)
 {
-    const auto kernel = prefix_own_kernel<BITS, G>;
+    const auto kernel = getenv("TOK32") ? prefix_own_kernel<BITS, G, 32> : prefix_own_kernel<BITS, G, 64>;
     if (plan.ctas) return launch_beside(kernel, B * ka.Hkv, 64, s, ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
     kernel<<<B * ka.Hkv, 64, 0, s>>>(ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
     return launch_status();
