@@ -134,12 +134,15 @@ def _load_host():
     spec = importlib.util.spec_from_file_location("_adkv_pyhost", _build.HOST_LIB)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    mod.bind(ctypes.cast(load().adkv_decode_attn, c_void_p).value)
+    lib = load()
+    mod.bind(ctypes.cast(lib.adkv_decode_attn, c_void_p).value)
+    mod.bind_more(*(ctypes.cast(f, c_void_p).value for f in (lib.adkv_decode_attn_prefix, lib.adkv_decode_attn_prefix_scratch_bytes,
+                                                             lib.adkv_norm_rope_qkv, lib.adkv_process_logits)))
     return mod
 
 
 def host():
-    """The native host module of ``gemv.decode_attn``, bound to the loaded library; False where it does not load (the
+    """The native host module of ``gemv.decode_attn`` and the calls of ``step``, bound to the loaded library; False where it does not load (the
     Python code does the same with more time per call), decided by the first call."""
     global _host
     if _host is None:

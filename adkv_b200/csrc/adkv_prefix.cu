@@ -17,7 +17,6 @@
 #include "adkv_host.h"
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "adkv_softmax.cuh"
 #include "adkv_tensor.cuh"
@@ -725,9 +724,12 @@ static int launch_beside(void (*kernel)(Params...), int grid, int block, cudaStr
 
 template <int BITS, int G>
 static int launch_own(const KArgs &ka, const VArgs &va, const float *k_state, const float *v_state, const int *seq_lens, float scaling,
-                      float *scratch, const PrefixPlan &plan, int B, cudaStream_t s)
+                      float *scratch, const PrefixPlan &plan, int B, int most, cudaStream_t s)
 {
-    const auto kernel = getenv("TOK32") ? prefix_own_kernel<BITS, G, 32> : prefix_own_kernel<BITS, G, 64>;
+    // Tiles of 32 tokens where a sequence is short, and with eight query heads, 4-bit, where 64 leave room for fewer CTAs (see short_tiles in
+    // adkv_fused.cu).  Whole step behind 64 tokens, 64 -> 32 tokens a tile: 64 x 32 heads, 100 tokens 32.2 -> 31.2 us, 600 81.9 -> 81.9 us; 32 x 8 of four
+    // heads, 2-bit, 100 20.5 -> 19.9 us, 600 56.4 -> 60.9 us; 128 x 8 of eight heads 100 49.0 -> 42.4 us, 600 118.9 -> 114.2 us, 1500 243 -> 252 us.
+    const auto kernel = most <= (BITS == 4 && G == 8 ? 1000 : 128) ? prefix_own_kernel<BITS, G, 32> : prefix_own_kernel<BITS, G, 64>;
     if (plan.ctas) return launch_beside(kernel, B * ka.Hkv, 64, s, ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
     kernel<<<B * ka.Hkv, 64, 0, s>>>(ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
     return launch_status();
@@ -802,9 +804,10 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     const PrefixPlan plan = prefix_plan(P, iv, B, G, Hkv);
     if (plan.ctas)
         if (int rc = bits == 4 ? launch_prefix<4>(pa, plan, s) : launch_prefix<2>(pa, plan, s)) return rc;
+    const int most = seq_lens ? int(std::min((long long)n_super_cap * (32 / bits), 1ll << 30)) : T;   // own tokens of a sequence, at most
     int rc = 0;
     ADKV_DISPATCH_H(bits, G, (rc = launch_own<BITS, G>(ka, va, static_cast<const float *>(prefix->k_tail), static_cast<const float *>(prefix->v_tail),
-                                                         static_cast<const int *>(seq_lens), scaling, pa.scratch, plan, B, s)))
+                                                         static_cast<const int *>(seq_lens), scaling, pa.scratch, plan, B, most, s)))
     if (rc) return rc;
     return launch_beside(prefix_join_kernel, B * Hq, 32 * kJoinWarps, s, pa.scratch, static_cast<__half *>(out), Hq, Hkv, plan);
 }

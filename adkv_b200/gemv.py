@@ -627,6 +627,7 @@ class SharedPrefix:
         self.k_tail, self.v_tail = k_tail, v_tail
         self._keep = (k_cache, v_cache, k_ckpt, v_ckpt)
         self.desc = _lib.Prefix(k_cache.data_ptr(), v_cache.data_ptr(), kt, vt, kc, vc, self.tokens, n_super_cap, self.interval, cap)
+        self._native = (ctypes.addressof(self.desc), H, bits, self.device.index)
 
     def start_tails(self, B: int):
         """Tail states ``[B, nh_kv, 2, DIM]`` of K and V for B sequences that have no tokens of their own yet."""
@@ -655,6 +656,14 @@ def decode_attn_prefix(q, prefix: SharedPrefix, k_cache, v_cache, k_new, v_new, 
     ``scratch`` (at least :func:`prefix_scratch_bytes`) is allocated per call when not given; two steps that may overlap on the GPU,
     captured graphs among them, must not share one."""
     _require(isinstance(prefix, SharedPrefix), "prefix must be a SharedPrefix")
+    native = _lib.host()
+    if native:                                  # plain contiguous tensors: checked and called in native code
+        done = native.decode_prefix(q, prefix._native, k_cache, v_cache, k_new, v_new, k_params, v_params, T, scaling, scale_min, scale_max, k_tail,
+                                    v_tail, _lib.flags(True, tail_keep=tail_keep), out, scratch)
+        if done is not None:
+            if isinstance(done, int):
+                _lib.check(done, "decode_attn_prefix")
+            return done
     _require(q.dtype == torch.float16, "q must be float16")
     _require(k_new.dtype == torch.float16 and v_new.dtype == torch.float16, "k_new / v_new must be float16")
     B, Hkv, n_super_cap, D = _cache_dims(k_cache, "k_cache")

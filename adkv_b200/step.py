@@ -33,6 +33,13 @@ def norm_rope_qkv(qkv, n_heads: int, n_kv_heads: int, cos, sin, *, start: int = 
     ``(i, i + rot / 2)``, or ``(2i, 2i + 1)`` if ``interleaved``; the others pass through.  Token t of a sequence is at position
     ``start + t``, or ``positions[b] + t`` / ``positions[b, t]`` for int32 CUDA tensors ``[B]`` / ``[B, T]``; a position on the device that has
     no row makes queries and keys of its token NaN and ``gemv.device_status`` report 8.  Computed in float32, rounded once at the end."""
+    native = _lib.host()
+    if native:                                  # plain tensors of the usual layouts: checked and called in native code
+        done = native.norm_rope(qkv, n_heads, n_kv_heads, cos, sin, start, positions, q_weight, k_weight, eps, interleaved, dtype)
+        if done is not None:
+            if isinstance(done, int):
+                _lib.check(done, "norm_rope_qkv")
+            return done
     _require(qkv.is_cuda, "qkv must be a CUDA tensor (adkv_b200 has no CPU path)")
     _require(qkv.dim() == 3 and qkv.dtype in _TYPES, "qkv must be float16, bfloat16 or float32 [B, T, (nh + 2 nh_kv) * DIM]")
     _require(n_heads > 0 and n_kv_heads > 0 and qkv.shape[2] % (n_heads + 2 * n_kv_heads) == 0, "qkv does not divide into its heads")
@@ -94,6 +101,13 @@ def process_logits(logits, *, history: torch.Tensor | None = None, history_lens:
 
     ``out``: of the logits' type and shape, may be ``logits`` itself.  ``tokens`` int32 ``[B]``: the lowest index of the largest element of
     ``out`` (a NaN counts as the largest), -1 for a row of nothing but -inf."""
+    native = out is None and _lib.host()
+    if native:                                  # as in norm_rope_qkv
+        done = native.logits(logits, history, history_lens, repetition, presence, frequency, bias, mask)
+        if done is not None:
+            if isinstance(done, int):
+                _lib.check(done, "process_logits")
+            return done
     _require(logits.is_cuda, "logits must be a CUDA tensor (adkv_b200 has no CPU path)")
     _require(logits.dim() == 2 and logits.dtype in _TYPES and logits.shape[1] > 0, "logits must be float16, bfloat16 or float32 [B, V]")
     B, V = logits.shape
