@@ -6,30 +6,49 @@
 
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 namespace adkv {
 
 constexpr int kStatPosition = 8;   // a position held on the device lies outside the rotation tables
 
-// Four consecutive elements of a row, as floats.
-__device__ __forceinline__ void load4(float (&v)[4], const __half *p) { load_half4(v, p); }
-__device__ __forceinline__ void load4(float (&v)[4], const __nv_bfloat16 *p)
-{
-    const uint2 a = *reinterpret_cast<const uint2 *>(p);
-    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
-    v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
-}
-__device__ __forceinline__ void load4(float (&v)[4], const float *p)
-{
-    const float4 a = *reinterpret_cast<const float4 *>(p);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-}
-__device__ __forceinline__ void store4(__half *p, const float (&v)[4]) { store_half4(p, v); }
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&v)[4])
-{
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-}
-__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+// Four consecutive elements of a row as they lie in memory, and as floats.
+template <class T>
+struct Four;
+template <>
+struct Four<__half> {
+    using Raw = uint2;
+    __device__ static void get(float (&v)[4], const uint2 &a)
+    {
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&a.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&a.y));
+        v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+    }
+    __device__ static uint2 put(const float (&v)[4])
+    {
+        const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    }
+};
+template <>
+struct Four<__nv_bfloat16> {
+    using Raw = uint2;
+    __device__ static void get(float (&v)[4], const uint2 &a)
+    {
+        v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+        v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+    }
+    __device__ static uint2 put(const float (&v)[4])
+    {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    }
+};
+template <>
+struct Four<float> {
+    using Raw = float4;
+    __device__ static void get(float (&v)[4], const float4 &a) { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
+    __device__ static float4 put(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
+};
 
 // =========================================================================================
 // Rotation of queries and keys, with the root-mean-square norm of each head before it:
@@ -40,8 +59,9 @@ __device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *reinter
 //
 // Bound by memory: every element is read and written once, the tables are 1 % of it.  A lane holds eight channels of a head, four
 // pairs, so that both halves of a pair are its own and nothing but the sum of squares crosses lanes; D / 8 lanes share a head, and a
-// thread takes the same channels of up to kRopeRows heads of one token, so cosines and sines are loaded once for them and their
-// loads are in flight together.
+// thread takes the same channels of up to kRopeRows heads of one token, so cosines and sines are loaded once for them.  A CTA goes on
+// from token to token, and the next two are on their way to shared memory while it works on one: with a token a CTA, half of the time
+// nothing is.  Every thread reads what it has copied itself, so nothing has to be waited for but its own copies.
 struct RopeArgs {
     const void *qkv;
     long long stride_b, stride_t;      // elements
@@ -50,113 +70,184 @@ struct RopeArgs {
     const float *cos, *sin;            // [table_rows, >= rot / 2]
     const int *positions;              // [B] (per_token false: of the first token) or [B, T], or nullptr
     long long table_stride;
-    int table_rows, rot, per_token, start, T, Hq, Hkv, interleaved;
+    int table_rows, rot, per_token, start, tokens, T, Hq, Hkv, interleaved;
+    int rows;                          // heads of a thread, at most kRopeRows
     float eps;
 };
 constexpr int kRopeThreads = 256, kRopeRows = 4;
+
+template <int D, class In>
+__host__ __device__ constexpr int rope_slot_bytes() { return kRopeRows * (D == 512 ? 2 : 1) * 2 * kRopeThreads * int(sizeof(typename Four<In>::Raw)); }   // of a stage
+template <int D, class In>
+__host__ __device__ constexpr int rope_stages() { return rope_slot_bytes<D, In>() > 32768 ? 2 : 3; }
+__device__ __forceinline__ void copy_async(uint2 *dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory"); }
+__device__ __forceinline__ void copy_async(float4 *dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory"); }
 
 template <int D, class In, class Out>
 __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ RopeArgs a)
 {
     constexpr int UNITS = D == 512 ? 2 : 1, LANES = D / 8 / UNITS;   // lanes of a head, and groups of eight channels of a lane
     constexpr int HEADS = kRopeThreads / LANES;                      // heads that the CTA takes side by side
-    const int token = blockIdx.x, b = token / a.T, t = token % a.T;
+    using Raw = typename Four<In>::Raw;
     const int lane = threadIdx.x % LANES, H = a.Hq + 2 * a.Hkv, half = a.rot / 2;
-    int pos = a.start + t;
-    if (a.positions) pos = a.per_token ? a.positions[token] : a.positions[b] + t;
-    const bool inside = pos >= 0 && pos < a.table_rows;
-    if (!inside && threadIdx.x == 0 && blockIdx.y == 0) atomicExch(&g_status, kStatPosition);
+    const int h0 = blockIdx.y * HEADS * a.rows + threadIdx.x / LANES;
 
     // first channels of the lane's two groups of four: pairs (first, second), or channels that are left as they are
     int at0[UNITS], at1[UNITS];
-    float c[UNITS][4], s[UNITS][4];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int pair = 4 * (lane + LANES * u);
-        const bool turned = pair < half, split = turned && !a.interleaved;
+        const bool split = pair < half && !a.interleaved;
         at0[u] = split ? pair : 2 * pair;
         at1[u] = split ? pair + half : 2 * pair + 4;
-        if (turned) {
-            const float bad = __int_as_float(0x7fc00000);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[u][i] = inside ? a.cos[(long long)pos * a.table_stride + pair + i] : bad;
-                s[u][i] = inside ? a.sin[(long long)pos * a.table_stride + pair + i] : bad;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { c[u][i] = inside ? 1.f : __int_as_float(0x7fc00000); s[u][i] = 0.f; }
-        }
     }
-    const In *src = static_cast<const In *>(a.qkv) + b * a.stride_b + t * a.stride_t;
-    const int h0 = blockIdx.y * HEADS * kRopeRows + threadIdx.x / LANES;
-    float x[kRopeRows][UNITS][2][4];
+    constexpr int ST = rope_stages<D, In>();
+    extern __shared__ __align__(16) uint8_t rope_smem[];
+    // stage, row, group of the lane's channels, half: the thread's own slot
+    const auto slot = [&](int st, int r, int u, int k) {
+        return reinterpret_cast<Raw *>(rope_smem) + (((st * kRopeRows + r) * UNITS + u) * 2 + k) * kRopeThreads + threadIdx.x;
+    };
+    // a token as its sequence and its place there, and the step from one of the CTA's tokens to the next
+    struct Place {
+        int b, t;
+    };
+    const int step_b = int(gridDim.x) / a.T, step_t = int(gridDim.x) % a.T;
+    const auto advance = [&](Place &p) {
+        p.b += step_b;
+        p.t += step_t;
+        if (p.t >= a.T) { p.t -= a.T; ++p.b; }
+    };
+    const int B = a.tokens / a.T;
+    const auto load = [&](const Place &p, int st) {
+        if (p.b < B) {
+            const In *src = static_cast<const In *>(a.qkv) + p.b * a.stride_b + p.t * a.stride_t + h0 * D;
 #pragma unroll
-    for (int r = 0; r < kRopeRows; ++r)
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int h = h0 + HEADS * r;
-            if (h < H) {
-                load4(x[r][u][0], src + h * D + at0[u]);
-                load4(x[r][u][1], src + h * D + at1[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[r][u][0][i] = x[r][u][1][i] = 0.f;
-            }
-        }
-#pragma unroll
-    for (int r = 0; r < kRopeRows; ++r) {
-        const int h = h0 + HEADS * r;
-        const bool is_v = h >= a.Hq + a.Hkv;
-        const In *weight = static_cast<const In *>(h < a.Hq ? a.q_weight : a.k_weight);
-        const bool norm = !is_v && weight;
-        if (a.q_weight || a.k_weight) {   // the same for all: the lanes of other heads take part in the sum
-            float sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(x[r][u][i / 4][i % 4], x[r][u][i / 4][i % 4], sum);
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-            if (norm) {
-                const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+            for (int r = 0; r < kRopeRows; ++r) {
+                if (r >= a.rows || h0 + HEADS * r >= H) break;
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
-                    float w0[4], w1[4];
-                    load4(w0, weight + at0[u]);
-                    load4(w1, weight + at1[u]);
+                    copy_async(slot(st, r, u, 0), src + HEADS * r * D + at0[u]);
+                    copy_async(slot(st, r, u, 1), src + HEADS * r * D + at1[u]);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const bool q_norm = a.q_weight, k_norm = a.k_weight, whole = a.table_stride % 4 == 0 && a.rot % 8 == 0 &&
+               ((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15) == 0;   // cosines and sines four at a time
+    Raw weight[2][UNITS][2] = {};   // of queries and keys
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        if (q_norm) {
+            weight[0][u][0] = *reinterpret_cast<const Raw *>(static_cast<const In *>(a.q_weight) + at0[u]);
+            weight[0][u][1] = *reinterpret_cast<const Raw *>(static_cast<const In *>(a.q_weight) + at1[u]);
+        }
+        if (k_norm) {
+            weight[1][u][0] = *reinterpret_cast<const Raw *>(static_cast<const In *>(a.k_weight) + at0[u]);
+            weight[1][u][1] = *reinterpret_cast<const Raw *>(static_cast<const In *>(a.k_weight) + at1[u]);
+        }
+    }
+    const auto finish = [&](const Place &p, int st) {
+        int pos = a.start + p.t;
+        if (a.positions) pos = a.per_token ? a.positions[p.b * a.T + p.t] : a.positions[p.b] + p.t;
+        float c[UNITS][4], s[UNITS][4];
+        const bool inside = pos >= 0 && pos < a.table_rows;
+        if (!inside && threadIdx.x == 0 && blockIdx.y == 0) atomicExch(&g_status, kStatPosition);
+        const float *cos = a.cos + (long long)pos * a.table_stride, *sin = a.sin + (long long)pos * a.table_stride;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int pair = 4 * (lane + LANES * u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[u][i] = inside ? 1.f : __int_as_float(0x7fc00000);
+                s[u][i] = 0.f;
+            }
+            if (inside && pair < half) {
+                if (whole) {
+                    Four<float>::get(c[u], *reinterpret_cast<const float4 *>(cos + pair));
+                    Four<float>::get(s[u], *reinterpret_cast<const float4 *>(sin + pair));
+                } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[r][u][0][i] *= inv * w0[i];
-                        x[r][u][1][i] *= inv * w1[i];
+                        c[u][i] = cos[pair + i];
+                        s[u][i] = sin[pair + i];
                     }
                 }
             }
         }
-        if (h >= H) continue;
-        Out *dst = is_v ? static_cast<Out *>(a.v) + (((long long)b * a.Hkv + h - a.Hq - a.Hkv) * a.T + t) * D
-                        : h < a.Hq ? static_cast<Out *>(a.q) + (((long long)b * a.Hq + h) * a.T + t) * D
-                                   : static_cast<Out *>(a.k) + (((long long)b * a.Hkv + h - a.Hq) * a.T + t) * D;
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            float(&p)[4] = x[r][u][0], (&n)[4] = x[r][u][1];
-            const auto turn = [](float &first, float &second, float co, float si) {
-                const float was = first;
-                first = __fsub_rn(__fmul_rn(was, co), __fmul_rn(second, si));
-                second = __fadd_rn(__fmul_rn(second, co), __fmul_rn(was, si));
-            };
-            if (!is_v) {
-                if (a.interleaved) {
-                    turn(p[0], p[1], c[u][0], s[u][0]); turn(p[2], p[3], c[u][1], s[u][1]);
-                    turn(n[0], n[1], c[u][2], s[u][2]); turn(n[2], n[3], c[u][3], s[u][3]);
-                } else {
+        for (int r = 0; r < kRopeRows; ++r) {
+            if (r >= a.rows) break;
+            const int h = h0 + HEADS * r;
+            const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+            float x[UNITS][2][4];   // of lanes behind the last head: whatever the slot holds, not used
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) turn(p[i], n[i], c[u][i], s[u][i]);
+            for (int u = 0; u < UNITS; ++u) {
+                Four<In>::get(x[u][0], *slot(st, r, u, 0));
+                Four<In>::get(x[u][1], *slot(st, r, u, 1));
+            }
+            if (q_norm || k_norm) {   // the same for all: the lanes of other heads take part in the sum
+                float sum = 0.f;
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i / 4][i % 4], x[u][i / 4][i % 4], sum);
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+                if (!is_v && (is_q ? q_norm : k_norm)) {
+                    const float inv = rsqrtf(sum * (1.f / D) + a.eps);
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float w[4];
+                            Four<In>::get(w, is_q ? weight[0][u][k] : weight[1][u][k]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[u][k][i] *= inv * w[i];
+                        }
                 }
             }
-            store4(dst + at0[u], p);
-            store4(dst + at1[u], n);
+            if (h >= H) continue;
+            // heads of the tensor and the head in it
+            const int n = is_q ? a.Hq : a.Hkv, at = is_q ? h : is_v ? h - a.Hq - a.Hkv : h - a.Hq;
+            Out *dst = static_cast<Out *>(is_q ? a.q : is_v ? a.v : a.k) + ((size_t(p.b) * n + at) * a.T + p.t) * D;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                float(&p)[4] = x[u][0], (&n)[4] = x[u][1];
+                const auto turn = [](float &first, float &second, float co, float si) {
+                    const float was = first;
+                    first = __fsub_rn(__fmul_rn(was, co), __fmul_rn(second, si));
+                    second = __fadd_rn(__fmul_rn(second, co), __fmul_rn(was, si));
+                };
+                if (!is_v) {
+                    if (a.interleaved) {
+                        turn(p[0], p[1], c[u][0], s[u][0]); turn(p[2], p[3], c[u][1], s[u][1]);
+                        turn(n[0], n[1], c[u][2], s[u][2]); turn(n[2], n[3], c[u][3], s[u][3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) turn(p[i], n[i], c[u][i], s[u][i]);
+                    }
+                }
+                using OutRaw = typename Four<Out>::Raw;
+                *reinterpret_cast<OutRaw *>(dst + at0[u]) = Four<Out>::put(p);
+                *reinterpret_cast<OutRaw *>(dst + at1[u]) = Four<Out>::put(n);
+            }
         }
+    };
+    Place now{int(blockIdx.x) / a.T, int(blockIdx.x) % a.T}, ahead = now;
+    int st = 0;
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k) {
+        load(ahead, k);
+        advance(ahead);
+    }
+#pragma unroll 1
+    for (; now.b < B; advance(now)) {
+        load(ahead, (st + ST - 1) % ST);
+        advance(ahead);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        finish(now, st);
+        st = st + 1 == ST ? 0 : st + 1;
     }
 }
 
@@ -386,20 +477,34 @@ using namespace adkv;
 
 ADKV_DEFINE_TU_STATUS(adkv_tu_status_step)
 
-template <int D>
-static int launch_rope(const RopeArgs &a, int B, int in_type, int out_type, cudaStream_t s)
+// CTAs that the chip holds of the kernel, four an SM.
+constexpr long long kRopePlaces = 4 * kSMs;
+
+template <int D, class In, class Out>
+static int launch_rope_kernel(const RopeArgs &a, dim3 grid, cudaStream_t s)
 {
-    constexpr int heads = kRopeThreads / (D / 8 / (D == 512 ? 2 : 1)) * kRopeRows;
-    const dim3 grid(unsigned(B) * unsigned(a.T), (a.Hq + 2 * a.Hkv + heads - 1) / heads);
+    constexpr int bytes = rope_stages<D, In>() * rope_slot_bytes<D, In>();
+    const auto kernel = norm_rope_kernel<D, In, Out>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return launch_status();
+    kernel<<<grid, kRopeThreads, bytes, s>>>(a);
+    return launch_status();
+}
+
+template <int D>
+static int launch_rope(RopeArgs a, int in_type, int out_type, cudaStream_t s)
+{
+    constexpr int heads = kRopeThreads / (D / 8 / (D == 512 ? 2 : 1));
+    const int each = (a.Hq + 2 * a.Hkv + heads - 1) / heads, groups = (each + kRopeRows - 1) / kRopeRows;
+    a.rows = (each + groups - 1) / groups;
+    const dim3 grid(std::min((long long)a.tokens, std::max(1ll, kRopePlaces / groups)), groups);
     switch (in_type * 4 + out_type) {
-    case ADKV_T_F16 * 4 + ADKV_T_F16: norm_rope_kernel<D, __half, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
-    case ADKV_T_BF16 * 4 + ADKV_T_F16: norm_rope_kernel<D, __nv_bfloat16, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
-    case ADKV_T_BF16 * 4 + ADKV_T_BF16: norm_rope_kernel<D, __nv_bfloat16, __nv_bfloat16><<<grid, kRopeThreads, 0, s>>>(a); break;
-    case ADKV_T_F32 * 4 + ADKV_T_F16: norm_rope_kernel<D, float, __half><<<grid, kRopeThreads, 0, s>>>(a); break;
-    case ADKV_T_F32 * 4 + ADKV_T_F32: norm_rope_kernel<D, float, float><<<grid, kRopeThreads, 0, s>>>(a); break;
+    case ADKV_T_F16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __half, __half>(a, grid, s);
+    case ADKV_T_BF16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __nv_bfloat16, __half>(a, grid, s);
+    case ADKV_T_BF16 * 4 + ADKV_T_BF16: return launch_rope_kernel<D, __nv_bfloat16, __nv_bfloat16>(a, grid, s);
+    case ADKV_T_F32 * 4 + ADKV_T_F16: return launch_rope_kernel<D, float, __half>(a, grid, s);
+    case ADKV_T_F32 * 4 + ADKV_T_F32: return launch_rope_kernel<D, float, float>(a, grid, s);
     default: return ADKV_E_TYPE;
     }
-    return launch_status();
 }
 
 static bool aligned_to(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -452,13 +557,13 @@ int adkv_norm_rope_qkv(const void *qkv, long long stride_b, long long stride_t, 
     if (!positions && B && T && (long long)start + T > table_rows) return ADKV_E_CAPACITY;
     if (B == 0 || T == 0) return 0;
     const RopeArgs a{qkv, stride_b, stride_t, q, k, v, q_weight, k_weight, static_cast<const float *>(cos), static_cast<const float *>(sin),
-                     static_cast<const int *>(positions), table_stride, table_rows, rot, positions_per_token, start, T, Hq, Hkv, interleaved, eps};
+                     static_cast<const int *>(positions), table_stride, table_rows, rot, positions_per_token, start, B * T, T, Hq, Hkv, interleaved, 0, eps};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (D) {
-    case 64: return launch_rope<64>(a, B, in_type, out_type, s);
-    case 128: return launch_rope<128>(a, B, in_type, out_type, s);
-    case 256: return launch_rope<256>(a, B, in_type, out_type, s);
-    default: return launch_rope<512>(a, B, in_type, out_type, s);
+    case 64: return launch_rope<64>(a, in_type, out_type, s);
+    case 128: return launch_rope<128>(a, in_type, out_type, s);
+    case 256: return launch_rope<256>(a, in_type, out_type, s);
+    default: return launch_rope<512>(a, in_type, out_type, s);
     }
 }
 
