@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
 //
 // Bound by memory for a batch, by latency for one row.  A cluster of up to eight CTAs shares a row; each counts the history's tokens
 // that fall into its part in shared memory (integer additions, so the order does not matter) and then passes over its part once, 16
-// aligned bytes a load whatever the row's alignment; the CTAs' largest values meet in the shared memory of the first, so nothing
-// has to be cleared, kept or launched besides.
+// aligned bytes a load whatever the row's alignment.  The first loads are under way while the history is counted.  The CTAs' largest
+// values meet in the shared memory of the first, so nothing has to be cleared, kept or launched besides.
 struct LogitArgs {
     const void *x;
     void *out;
@@ -272,9 +272,10 @@ struct LogitArgs {
     const uint32_t *mask;                                    // [B, >= (V + 31) / 32], or nullptr
     long long stride_x, stride_out, stride_history, stride_bias, stride_mask;
     int V, history_cap;
-    int part;                                                // packs of a CTA, see below
+    int part;                                                // packs of a CTA, a multiple of 32, see below
 };
-constexpr int kLogitThreads = 512, kLogitChunk = 14336, kLogitCluster = 8;   // tokens counted at a time: 56 KB
+constexpr int kLogitThreads = 512, kLogitCluster = 8, kLogitAhead = 4;   // kLogitAhead: loads of a thread that are under way at once
+constexpr int kLogitBytes = 73728;                                       // of counts
 
 template <class T>
 struct LogitIo;
@@ -347,21 +348,29 @@ struct LogitIo<__nv_bfloat16> {
 };
 
 // Value and index as one number whose order is that of the choice: larger values first (NaN above all, -0 as +0), then lower indexes.
-__device__ __forceinline__ unsigned long long rank_of(float v, int index)
+__device__ __forceinline__ uint32_t key_of(float v)
 {
     const uint32_t u = __float_as_uint(v + 0.f);
-    const uint32_t key = v != v ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
-    return (unsigned long long)key << 32 | uint32_t(~index);
+    return v != v ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
 }
+__device__ __forceinline__ unsigned long long rank_of(float v, int index) { return (unsigned long long)key_of(v) << 32 | uint32_t(~index); }
 constexpr uint32_t kRankMinusInf = 0x007fffffu;   // key of -inf
 
+__device__ __forceinline__ float max_or_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // A pack: the elements of 16 aligned bytes of the row.  A row that starts `skew` elements behind such a boundary has elements
-// p * N - skew ... of pack p; of the first and the last one some lie outside.
-template <class T>
-__global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(const __grid_constant__ LogitArgs a)
+// p * N - skew ... of pack p; of the first and the last one some lie outside.  Count: what an occurrence is counted in, 16 bits where a
+// history is short enough for it.
+template <class T, class Count>
+__global__ void __launch_bounds__(kLogitThreads, 2) process_logits_kernel(const __grid_constant__ LogitArgs a)
 {
     using Io = LogitIo<T>;
-    constexpr int N = Io::N;
+    constexpr int N = Io::N, PER = 4 / int(sizeof(Count));   // counts in a word
     extern __shared__ __align__(16) uint32_t counts[];
     __shared__ unsigned long long best[kLogitThreads / 32], gathered[kLogitCluster];
     uint32_t rank, ranks;
@@ -377,83 +386,151 @@ __global__ void __launch_bounds__(kLogitThreads) process_logits_kernel(const __g
     const int n_words = (a.V + 31) / 32;
     const int skew = int(reinterpret_cast<uintptr_t>(x) / sizeof(T) % N);
     const bool same = int(reinterpret_cast<uintptr_t>(out) / sizeof(T) % N) == skew;   // else the results are stored one by one
-    const int packs = (a.V + skew + N - 1) / N, p_end = min(packs, int(rank + 1) * a.part);
+    const bool bias4 = (reinterpret_cast<uintptr_t>(bias) / 4 - skew) % 4 == 0;        // four biases a load
+    const int packs = (a.V + skew + N - 1) / N;
+    // A row's packs are dealt out 32 at a time, so that every CTA of the cluster gets its share of the frequent tokens, which have the
+    // low numbers.  Its l-th pack is number
+    const int log_ranks = __ffs(ranks) - 1;
+    const auto pack_of = [&](int l) { return ((l >> 5 << log_ranks | int(rank)) << 5) | (l & 31); };
     const float rep = a.repetition ? a.repetition[b] : a.repetition1, pres = a.presence ? a.presence[b] : a.presence1,
                 freq = a.frequency ? a.frequency[b] : a.frequency1;
     const int *history = a.history ? a.history + b * a.stride_history : nullptr;
     const int n_history = !history ? 0 : a.history_lens ? min(max(a.history_lens[b], 0), a.history_cap) : a.history_cap;
 
-    unsigned long long top = 0;
-    constexpr int kPacks = kLogitChunk / N;
-    for (int p0 = int(rank) * a.part; p0 < p_end; p0 += kPacks) {
-        const int p1 = min(p_end, p0 + kPacks), v0 = p0 * N - skew;
+    const auto whole = [&](int p) { return p * N >= skew && p * N - skew + N <= a.V; };   // all of a pack lies in the row
+    uint32_t top_key = 0;
+    int top_at = a.V;
+    uint4 top_pack = make_uint4(0, 0, 0, 0);
+    constexpr int kPacks = kLogitBytes / int(sizeof(Count)) / N;
+    for (int p0 = 0; p0 < a.part; p0 += kPacks) {
+        const int p1 = min(a.part, p0 + kPacks);
+        uint4 ahead[kLogitAhead];
+        const auto fetch = [&](int l) {
+#pragma unroll
+            for (int u = 0; u < kLogitAhead; ++u) {
+                const int q = pack_of(l + u * kLogitThreads);
+                ahead[u] = l + u * kLogitThreads < p1 && whole(q) ? *reinterpret_cast<const uint4 *>(x + (q * N - skew)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        fetch(p0 + threadIdx.x);
         if (n_history) {
-            for (int i = threadIdx.x; i < (p1 - p0) * N / 4; i += kLogitThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
+            for (int i = threadIdx.x; i < ((p1 - p0) * N / PER + 3) / 4; i += kLogitThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
-            const uint32_t n = uint32_t((p1 - p0) * N);
+#pragma unroll 8
             for (int i = threadIdx.x; i < n_history; i += kLogitThreads) {
                 const int id = history[i];
-                if (id >= 0 && id < a.V && uint32_t(id - v0) < n) atomicAdd(&counts[id - v0], 1u);
+                const uint32_t e = uint32_t(id) + uint32_t(skew), group = e / (32 * N);
+                const int l = int(group >> log_ranks << 5 | (e / N & 31)) - p0;   // the CTA's pack that holds it, if it is the CTA's
+                if (id >= 0 && id < a.V && (group & (ranks - 1)) == rank && l >= 0 && l < p1 - p0) {
+                    const uint32_t at = uint32_t(l) * N + e % N;
+                    atomicAdd(&counts[at / PER], 1u << (at % PER * 16));
+                }
             }
             __syncthreads();
         }
-        for (int p = p0 + threadIdx.x; p < p1; p += kLogitThreads) {
-            const int v = p * N - skew;                    // index of the pack's first element
-            const bool whole = v >= 0 && v + N <= a.V;
-            float y[N];
-            if (whole) {
-                Io::unpack(*reinterpret_cast<const uint4 *>(x + v), y);
-            } else {
+        for (int base = p0 + threadIdx.x; base < p1; base += kLogitAhead * kLogitThreads) {
+            if (base >= p0 + kLogitAhead * kLogitThreads) fetch(base);
 #pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = v + i >= 0 && v + i < a.V ? Io::load(x + v + i) : 0.f;
-            }
-            if (n_history) {
-                uint32_t n[N], any = 0;
+            for (int u = 0; u < kLogitAhead; ++u) {
+                const int l = base + u * kLogitThreads, p = pack_of(l);
+                if (l >= p1 || p >= packs) break;
+                const int v = p * N - skew;                    // index of the pack's first element
+                const bool all = whole(p);
+                float y[N];
+                if (all) {
+                    Io::unpack(ahead[u], y);
+                } else {
 #pragma unroll
-                for (int i = 0; i < N; i += 4) {
-                    const uint4 c = *reinterpret_cast<const uint4 *>(counts + (p - p0) * N + i);
-                    n[i] = c.x; n[i + 1] = c.y; n[i + 2] = c.z; n[i + 3] = c.w;
-                    any |= c.x | c.y | c.z | c.w;
+                    for (int i = 0; i < N; ++i) y[i] = v + i >= 0 && v + i < a.V ? Io::load(x + v + i) : 0.f;
                 }
-                if (any) {
+                if (n_history) {
+                    uint32_t w[N / PER], any = 0;
+#pragma unroll
+                    for (int i = 0; i < N / PER; ++i) w[i] = 0;
+                    if constexpr (N / PER >= 4) {
+#pragma unroll
+                        for (int i = 0; i < N / PER; i += 4) {
+                            const uint4 c = *reinterpret_cast<const uint4 *>(counts + (l - p0) * (N / PER) + i);
+                            w[i] = c.x; w[i + 1] = c.y; w[i + 2] = c.z; w[i + 3] = c.w;
+                        }
+                    } else {
+                        const uint2 c = *reinterpret_cast<const uint2 *>(counts + (l - p0) * (N / PER));
+                        w[0] = c.x; w[1] = c.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < N / PER; ++i) any |= w[i];
+                    if (any) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const uint32_t n = PER == 1 ? w[i / PER] : w[i / PER] >> (i % PER * 16) & 0xffffu;
+                            if (n) {
+                                const float z = y[i] > 0.f ? __fdiv_rn(y[i], rep) : __fmul_rn(y[i], rep);
+                                y[i] = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(n)), pres));
+                            }
+                        }
+                    }
+                }
+                if (bias) {
+                    if (all && bias4) {
+#pragma unroll
+                        for (int i = 0; i < N; i += 4) {
+                            const float4 z = *reinterpret_cast<const float4 *>(bias + v + i);
+                            y[i] = __fadd_rn(y[i], z.x); y[i + 1] = __fadd_rn(y[i + 1], z.y);
+                            y[i + 2] = __fadd_rn(y[i + 2], z.z); y[i + 3] = __fadd_rn(y[i + 3], z.w);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+                            if (all || (v + i >= 0 && v + i < a.V)) y[i] = __fadd_rn(y[i], bias[v + i]);
+                    }
+                }
+                if (mask) {
+                    const int at = max(v, 0);
+                    const uint32_t w0 = mask[at >> 5], w1 = mask[min((at >> 5) + 1, n_words - 1)];
+                    const uint32_t bits = __funnelshift_r(w0, w1, at & 31) << (at - v);
 #pragma unroll
                     for (int i = 0; i < N; ++i)
-                        if (n[i]) {
-                            const float z = y[i] > 0.f ? __fdiv_rn(y[i], rep) : __fmul_rn(y[i], rep);
-                            y[i] = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(n[i])), pres));
-                        }
+                        if (!(bits >> i & 1)) y[i] = -INFINITY;
                 }
-            }
-            if (bias) {
+                const uint4 packed = Io::pack(y);
+                if (all && same) {
+                    *reinterpret_cast<uint4 *>(out + v) = packed;
+                } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (whole || (v + i >= 0 && v + i < a.V)) y[i] = __fadd_rn(y[i], bias[v + i]);
-            }
-            if (mask) {
-                const int at = max(v, 0);
-                const uint32_t w0 = mask[at >> 5], w1 = mask[min((at >> 5) + 1, n_words - 1)];
-                const uint32_t bits = __funnelshift_r(w0, w1, at & 31) << (at - v);
+                    for (int i = 0; i < N; ++i)
+                        if (v + i >= 0 && v + i < a.V) Io::store(out + v + i, y[i]);
+                }
+                if (a.tokens) {   // the pack with the largest element so far, the first of them (a thread's packs come in order)
+                    Io::unpack(packed, y);   // as they have been rounded
+                    if (!all) {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (!(bits >> i & 1)) y[i] = -INFINITY;
-            }
-            if (whole && same) {
-                *reinterpret_cast<uint4 *>(out + v) = Io::pack(y);
-            } else {
+                        for (int i = 0; i < N; ++i)
+                            if (v + i < 0 || v + i >= a.V) y[i] = -INFINITY;
+                    }
+                    float most = y[0];
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (v + i >= 0 && v + i < a.V) Io::store(out + v + i, y[i]);
-            }
-            if (a.tokens) {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (whole || (v + i >= 0 && v + i < a.V)) top = max(top, rank_of(Io::round(y[i]), v + i));
+                    for (int i = 1; i < N; ++i) most = max_or_nan(most, y[i]);
+                    const uint32_t key = key_of(most);
+                    if (key > top_key) {
+                        top_key = key;
+                        top_at = v;
+                        top_pack = packed;
+                    }
+                }
             }
         }
         __syncthreads();   // the counts are read
     }
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (!a.tokens) return;
+    unsigned long long top = 0;
+    {
+        float y[N];
+        Io::unpack(top_pack, y);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (top_at + i >= 0 && top_at + i < a.V) top = max(top, rank_of(y[i], top_at + i));
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
     if (threadIdx.x % 32 == 0) best[threadIdx.x / 32] = top;
@@ -509,19 +586,21 @@ static int launch_rope(RopeArgs a, int in_type, int out_type, cudaStream_t s)
 
 static bool aligned_to(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-template <class T>
-static int launch_logits(LogitArgs a, int B, cudaStream_t s)
+template <class T, class Count>
+static int launch_logits_kernel(LogitArgs a, int B, cudaStream_t s)
 {
-    constexpr int N = LogitIo<T>::N;
-    // CTAs of a row: more until the launch fills the chip twice over or a CTA has fewer than 2048 elements
+    constexpr int N = LogitIo<T>::N, room = kLogitBytes / int(sizeof(Count));   // tokens that can be counted at once
+    // CTAs of a row: more while the chip holds them all at once, two an SM, and each has 2048 elements, and while a CTA's part of a row
+    // with a history is more than it can count at once
     int cluster = 1;
-    while (cluster < kLogitCluster && (long long)B * cluster < 2 * kSMs && a.V / (2 * cluster) >= 2048) cluster *= 2;
-    while (cluster < kLogitCluster && a.history && a.V / cluster > kLogitChunk) cluster *= 2;   // each counts its part at once
+    while (cluster < kLogitCluster && 2ll * B * cluster <= 2 * kSMs && a.V / (2 * cluster) >= 2048) cluster *= 2;
+    while (cluster < kLogitCluster && a.history && a.V / cluster > room) cluster *= 2;
     const int packs = (a.V + 2 * N - 2) / N;   // of the worst alignment
-    a.part = (packs + cluster - 1) / cluster;
-    const int bytes = a.history ? min(a.part * N, kLogitChunk) * 4 : 0;
-    const auto kernel = process_logits_kernel<T>;
-    if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitChunk * 4) != cudaSuccess) return launch_status();
+    a.part = ((packs + 31) / 32 + cluster - 1) / cluster * 32;
+    const int bytes = a.history ? std::min((a.part * N * int(sizeof(Count)) + 15) / 16 * 16, kLogitBytes) : 0;
+    const auto kernel = process_logits_kernel<T, Count>;
+    if (bytes > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitBytes) != cudaSuccess)
+        return launch_status();
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = cluster;
@@ -535,6 +614,11 @@ static int launch_logits(LogitArgs a, int B, cudaStream_t s)
     cfg.numAttrs = 1;
     if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return launch_status();
     return launch_status();
+}
+template <class T>
+static int launch_logits(const LogitArgs &a, int B, cudaStream_t s)
+{
+    return a.history_cap > 65535 ? launch_logits_kernel<T, uint32_t>(a, B, s) : launch_logits_kernel<T, uint16_t>(a, B, s);
 }
 
 extern "C" {
