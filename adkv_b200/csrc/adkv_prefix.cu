@@ -10,10 +10,13 @@
 // memory.  A CTA takes 128 rows of one head and a run of checkpoint intervals (state checkpoints make runs independent), leaves maximum,
 // denominator and sums of each row in scratch memory, and the merge of adkv_split.cu joins them with the sequences' own parts.
 //
-// Values are rounded to fp16 for the products, as a cache of fp16 keys and values would hold them, but as differences from the zero
-// point at the start of the run: that point's share of a logit is the same for the whole run and is added in fp32 to the maximum, its
-// share of the result to the sums, so a channel far from zero keeps the bits of its deviations.  They are held in units of 16, a power
-// of two, so that differences up to a million are in range.  Weights are rounded to fp16, sums of both products are fp32.
+// Values are fp16 numbers for the products, as differences from the zero point at the start of the run: that point's share of a logit is
+// the same for the whole run and is added in fp32 to the maximum, its share of the result to the sums, so a channel far from zero keeps the
+// bits of its deviations.  They are held in units of 16, a power of two, so that differences up to a million are in range.  One fp16 number
+// is 2^-11 of a value: with channels that reach 50, as the outliers of this library's benchmark do, logits would be off by some 1e-3 and
+// results by up to 2.7 times what its results may be off (2e-3 and 2e-3 of the value), so K and V are pairs, rounded value and remainder
+// (22 bits), for two more products.  Weights are rounded to fp16, and the denominator adds them up as rounded, so that what a weight is
+// off cancels where it dominates; sums of all products are fp32.
 #include "adkv_host.h"
 
 #include <algorithm>
@@ -55,7 +58,8 @@ struct PrefixPlan {
 template <int BITS>
 struct PrefixShared {
     alignas(128) __half q[kD / 8][kPreRows][8];          // [channel / 8][row][channel % 8]
-    alignas(128) __half x[2][2][kPreTok / 8][kD][8];     // K, V; buffer; [token / 8][channel][token % 8]
+    // K, V; half of a tile: [token / 8][channel][token % 8], the rounded values in the first four rows and the remainders in the others
+    alignas(128) __half x[2][2][kPreTok / 8][kD][8];
     alignas(128) uint32_t words[2][2][kPreTok * BITS / 32][kD];   // packed tiles of K and V
     alignas(16) float z0[kD];                            // zero points of K before the run
     // The results of the run lie in x and what follows, a row every kPartStride floats (no two of eight in the same banks), and the zero
@@ -64,29 +68,24 @@ struct PrefixShared {
     __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][1][kPreTok * BITS / 32 - 1][0]); }
     uint32_t tmem;
     int dead;                                            // a bounded wait gave up
-    // of tile i, buffer i % 2: words are there; K and V values are there; S is there (and K has been read); weights are there; O is added up (V, P read)
-    uint64_t loaded[2][2], full[2][2], sdone[2], pfull[2], odone[2];
+    // of tile i, buffer i % 2: words are there; S is there; weights are there; O is added up (and the weights have been read)
+    uint64_t loaded[2][2], sdone[2], pfull[2], odone[2];
+    uint64_t full[2][2], read[2][2];                     // of K and V, halves of a tile: values are there, have been read
 };
 
 // K-major shared-memory matrix without swizzle: element (m, k) lies at (m / 8) * m_stride + (k / 8) * k_stride + (m % 8) * 16 + (k % 8) * 2.
 __device__ __forceinline__ uint64_t k_major_desc(const void *p, uint32_t k_stride, uint32_t m_stride) { return mn_major_desc(p, k_stride, m_stride); }
 // fp16 x fp16 -> fp32, A K-major; B K-major or N-major
-__host__ __device__ constexpr uint32_t pre_mma_desc(int M, int N, bool b_mn)
+__host__ __device__ constexpr uint32_t pre_mma_desc(int M, int N, bool b_mn, bool neg_a = false)
 {
-    return 1u << 4 | uint32_t(b_mn) << 16 | uint32_t(N >> 3) << 17 | uint32_t(M >> 4) << 24;
+    return 1u << 4 | uint32_t(neg_a) << 13 | uint32_t(b_mn) << 16 | uint32_t(N >> 3) << 17 | uint32_t(M >> 4) << 24;
 }
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // What one thread keeps of its channel, in units of kPreUnit; the zero point counts from the start of the run.
 struct PrefixChan {
     float zp, s, alpha, beta, tc;
 };
-// Eight tokens, fields 0..7 of w, contracted as in k_chunk2; the values go to dst.  GUARDED: with the eps guard, the clamps and the
+// Eight tokens, fields 0..7 of w, contracted as in k_chunk2; the values go to dst, the remainders behind.  GUARDED: with the eps guard, the clamps and the
 // end of the run (left tokens).  Otherwise least and most take in the scale before every fourth token, which tells afterwards whether
 // the guards would have done anything.
 template <int BITS, bool GUARDED>
@@ -109,7 +108,10 @@ __device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS
         c.s *= fmaf(c.beta, fabsf(q), c.tc);
         if (GUARDED) c.s = fminf(fmaxf(c.s, smin), smax);
     });
-    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    const uint4 hi = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+    *reinterpret_cast<uint4 *>(dst) = hi;
+    *reinterpret_cast<uint4 *>(dst + (kPreTok / 16) * kD * 16) = make_uint4(pack_remainder(hi.x, x[0], x[1]), pack_remainder(hi.y, x[2], x[3]),
+                                                                            pack_remainder(hi.z, x[4], x[5]), pack_remainder(hi.w, x[6], x[7]));
 }
 
 __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreSlack
@@ -117,6 +119,12 @@ __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
+}
+// v plus the halves of h
+__device__ __forceinline__ float add_halves(uint32_t h, float v)
+{
+    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tadd.rn.f32.f16 %0, x, %0;\n\tadd.rn.f32.f16 %0, y, %0;\n\t}" : "+f"(v) : "r"(h));
+    return v;
 }
 __device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane, int count = 1)
 {
@@ -160,8 +168,10 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.loaded[0][i], 1);
             mbar_init(&sh.loaded[1][i], 1);
-            mbar_init(&sh.full[0][i], 4);
-            mbar_init(&sh.full[1][i], 4);
+            for (int k = 0; k < 2; ++k) {
+                mbar_init(&sh.full[k][i], 4);
+                mbar_init(&sh.read[k][i], 1);
+            }
             mbar_init(&sh.sdone[i], 1);
             mbar_init(&sh.pfull[i], 4);
             mbar_init(&sh.odone[i], 1);
@@ -251,20 +261,19 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             const float hi = a.smax * (1.f / kPreUnit) / (gmx * gmx * gmx * gmx * (1.f + 2e-5f));
             PrefixChan ch{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f)};
             if (which == 0) sh.z0[c] = start;
-            uint64_t *freed = which ? sh.odone : sh.sdone;
             bool tame = true;   // no scale of the warp was outside its interval when last looked at
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i) {
                 const int tile = done + i, buf = tile & 1;
-                // the words have come, and the products that read this buffer before are done
-                if (!(ok = mbar_wait_both(&sh.loaded[which][buf], tile >> 1 & 1, tile >= 2 ? &freed[buf] : nullptr, (tile >> 1 & 1) ^ 1, kStatKWait))) break;
+                if (!(ok = mbar_wait(&sh.loaded[which][buf], tile >> 1 & 1, kStatKWait))) break;
                 const uint32_t *row = &sh.words[which][buf][0][c];
-                uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][buf][0][c][0]);
                 int left = ntok - i * kPreTok;
                 // Rounds of 32 tokens without guards first, which is right if every fourth scale was inside its interval: one vote a
                 // round.  Where it was not the round is done again with guards, and so are the next ones at once until it is.
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half, left -= kPreTok / 2, dst += (kPreTok / 16) * kD * 16) {
+                for (int half = 0; half < 2; ++half, left -= kPreTok / 2) {
+                    if (tile >= 1 && !(ok = mbar_wait(&sh.read[which][half], (tile & 1) ^ 1, kStatKWait))) break;
+                    uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][half][0][c][0]);
                     uint32_t w[WORDS / 2];
 #pragma unroll
                     for (int k = 0; k < WORDS / 2; ++k, row += kD) w[k] = *row;
@@ -298,9 +307,10 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                         }
                         tame = __all_sync(kFull, least >= lo && most <= hi);
                     }
+                    fence_async_shared();
+                    warp_arrive(&sh.full[which][half], lane);
                 }
-                fence_async_shared();
-                warp_arrive(&sh.full[which][buf], lane);
+                if (!ok) break;
             }
             if (which == 1) sh.z0_v()[c] = start;
             if (!ok && lane == 0) sh.dead = 1;
@@ -367,8 +377,8 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                                 p0 = n + j < left ? p0 : 0.f;
                                 p1 = n + j + 1 < left ? p1 : 0.f;
                             }
-                            l += p0 + p1;
-                            p[j / 2] = pack2(p0, p1);
+                            p[j / 2] = pack_half2(p0, p1);
+                            l = add_halves(p[j / 2], l);   // as they have been rounded: what a weight is off cancels where it dominates
                         }
                         tmem_st4(cols + n / 2, p[0], p[1], p[2], p[3]);
                         tmem_st4(cols + n / 2 + 4, p[4], p[5], p[6], p[7]);
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             }
         } else if (warp == 12) {
             // -------------------------------------------------------------------------- S = Q x^T
-            constexpr uint32_t desc = pre_mma_desc(kPreRows, kPreTok, true);
+            constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kPreTok / 2, true), lo_desc = pre_mma_desc(kPreRows, kPreTok / 2, true, true);
             int i = 0;
             int issued = min(2, n_tiles);
             if (elect_one())
@@ -443,20 +453,27 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
                 const int tile = done + i, buf = tile & 1;
-                if (!(ok = mbar_wait(&sh.full[0][buf], tile >> 1 & 1, kStatKWait))) break;
-                if (issued < n_tiles) {
+                if (tile >= 2 && !(ok = mbar_wait(&sh.odone[buf], (tile >> 1 & 1) ^ 1, kStatVWait))) break;   // the weights in S's place are used
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if (!(ok = mbar_wait(&sh.full[0][half], tile & 1, kStatKWait))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t d = tmem + kColS + kPreTok * buf + (kPreTok / 2) * half;
+                        const uint64_t qd = k_major_desc(&sh.q[0][0][0], kPreRows * 16, 128), xd = mn_major_desc(&sh.x[0][half][0][0][0], 128, kD * 16);
+#pragma unroll
+                        for (int n = 0; n < kD / 16; ++n) mma_smem(d, qd + 2 * kPreRows * n, xd + 16 * n, hi_desc, n > 0);
+#pragma unroll
+                        for (int n = 0; n < kD / 16; ++n) mma_smem(d, qd + 2 * kPreRows * n, xd + (kPreTok / 16) * kD + 16 * n, lo_desc, true);
+                        mma_commit(&sh.read[0][half]);
+                        if (half) mma_commit(&sh.sdone[buf]);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (issued < n_tiles) {   // the words of this tile are read
                     if (elect_one()) load_tile(0, issued);
                     ++issued;
-                }   // the words of this tile are read
-                __syncwarp();
-                if (tile >= 2 && !(ok = mbar_wait(&sh.odone[buf], (tile >> 1 & 1) ^ 1, kStatVWait))) break;   // the weights in S's place are used
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t qd = k_major_desc(&sh.q[0][0][0], kPreRows * 16, 128), xd = mn_major_desc(&sh.x[0][buf][0][0][0], 128, kD * 16);
-#pragma unroll
-                    for (int n = 0; n < kD / 16; ++n)
-                        mma_smem(tmem + kColS + kPreTok * buf, qd + 2 * kPreRows * n, xd + 16 * n, desc, n > 0);
-                    mma_commit(&sh.sdone[buf]);
                 }
                 __syncwarp();
             }
@@ -464,11 +481,12 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             __syncthreads();
             if (sh.dead) {   // products and copies in flight
                 for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k & 1], k >> 1 & 1, kStatDrain);
+                if (!ok) mbar_wait(&sh.read[0][0], done + i & 1, kStatDrain);   // the first half of the tile at which this warp gave up, if it was issued
                 for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k & 1], k >> 1 & 1, kStatDrain);
             }
         } else {
             // -------------------------------------------------------------------------- O += P y
-            constexpr uint32_t desc = pre_mma_desc(kPreRows, kD, false);
+            constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kD, false), lo_desc = pre_mma_desc(kPreRows, kD, false, true);
             int i = 0;
             int issued = min(2, n_tiles);
             if (elect_one())
@@ -478,20 +496,28 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
                 const int tile = done + i, buf = tile & 1;
-                if (!(ok = mbar_wait(&sh.full[1][buf], tile >> 1 & 1, kStatVWait))) break;
-                if (issued < n_tiles) {
+                if (!(ok = mbar_wait(&sh.pfull[buf], tile >> 1 & 1, kStatVWait))) break;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if (!(ok = mbar_wait(&sh.full[1][half], tile & 1, kStatVWait))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t pa = tmem + kColS + kPreTok * buf + (kPreTok / 4) * half;
+                        const uint64_t yd = k_major_desc(&sh.x[1][half][0][0][0], kD * 16, 128);
+#pragma unroll
+                        for (int n = 0; n < kPreTok / 32; ++n) {
+                            mma_tmem(tmem + kColO, pa + 8 * n, yd + 2 * kD * n, hi_desc, i > 0 || half > 0 || n > 0);
+                            mma_tmem(tmem + kColO, pa + 8 * n, yd + (kPreTok / 16) * kD + 2 * kD * n, lo_desc, true);
+                        }
+                        mma_commit(&sh.read[1][half]);
+                        if (half) mma_commit(&sh.odone[buf]);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (issued < n_tiles) {   // the words of this tile are read
                     if (elect_one()) load_tile(1, issued);
                     ++issued;
-                }
-                __syncwarp();
-                if (!(ok = mbar_wait(&sh.pfull[buf], tile >> 1 & 1, kStatVWait))) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t yd = k_major_desc(&sh.x[1][buf][0][0][0], kD * 16, 128);
-#pragma unroll
-                    for (int n = 0; n < kPreTok / 16; ++n)
-                        mma_tmem(tmem + kColO, tmem + kColS + kPreTok * buf + 8 * n, yd + 2 * kD * n, desc, i > 0 || n > 0);
-                    mma_commit(&sh.odone[buf]);
                 }
                 __syncwarp();
             }
@@ -499,6 +525,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             __syncthreads();
             if (sh.dead) {
                 for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.odone[k & 1], k >> 1 & 1, kStatDrain);
+                if (!ok) mbar_wait(&sh.read[1][0], done + i & 1, kStatDrain);
                 for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k & 1], k >> 1 & 1, kStatDrain);
             }
         }

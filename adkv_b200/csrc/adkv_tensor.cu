@@ -67,22 +67,6 @@ struct TensorShared {
     uint64_t loaded[2][ST], kfull[NB], kdone[NB], kread, lfull[NB], lread[NB], vfull[NB], wfull[NB], vdone[NB], vread[NB];
 };
 
-// two fp16 numbers
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-// the halves of h minus a and b, as fp16: the remainders with the sign turned (the products of this part subtract)
-__device__ __forceinline__ uint32_t pack_remainder(uint32_t h, float a, float b)
-{
-    float d0, d1;
-    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tsub.rn.f32.f16 %0, x, %2;\n\t}" : "=f"(d0) : "r"(h), "f"(a));
-    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tsub.rn.f32.f16 %0, y, %2;\n\t}" : "=f"(d1) : "r"(h), "f"(b));
-    return pack_half2(d0, d1);
-}
-
 // What one thread keeps of its channel.  The scale is held in units of a power of two below the upper bound, so that the fp16 parts
 // of the dequantised values have their bits where they are needed; scaling by it rounds nothing.
 struct TensorChan {

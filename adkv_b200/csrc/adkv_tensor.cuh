@@ -1,4 +1,4 @@
-// Tensor memory and tcgen05 wrappers (one CTA, kind::f16 with fp32 accumulators) of the decode kernel in adkv_tensor.cu.
+// Tensor memory and tcgen05 wrappers (one CTA, kind::f16 with fp32 accumulators) of the decode kernels in adkv_tensor.cu and adkv_prefix.cu.
 #pragma once
 #include "adkv_device.cuh"
 
@@ -51,6 +51,22 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
 __device__ __forceinline__ void mma_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// two fp16 numbers
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// the halves of h minus a and b, as fp16: the remainders with the sign turned (the products of this part subtract)
+__device__ __forceinline__ uint32_t pack_remainder(uint32_t h, float a, float b)
+{
+    float d0, d1;
+    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tsub.rn.f32.f16 %0, x, %2;\n\t}" : "=f"(d0) : "r"(h), "f"(a));
+    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tsub.rn.f32.f16 %0, y, %2;\n\t}" : "=f"(d1) : "r"(h), "f"(b));
+    return pack_half2(d0, d1);
 }
 
 // a warp's 32 lanes x N columns; finished at tmem_wait_ld / tmem_wait_st

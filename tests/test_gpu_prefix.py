@@ -105,12 +105,13 @@ class Shared:
         return out
 
     def want(self, scaling=SCALING):
-        """Result in float64, and a bound of what fp16 operands and fp32 sums may add to it.
+        """Result in float64, and a bound of what the operands of the products and fp32 sums may add to it.
 
-        Values of the prefix are rounded to fp16 as differences from the zero point at the start of a run, a step of at most 2^-10 of the
-        difference, or 2^-20 (units of 16): the error of a logit is a sum of D independent roundings, each uniform in half a step, and is
-        taken at eight standard deviations.  Runs may span intervals, so differences count from any interval's start.  Replays in 32 bits
-        are off by at most 8 roundings of the largest value a token, weights by half a step of fp16 each, and the result by half a step."""
+        Values of the prefix are pairs of fp16 numbers, as differences from the zero point at the start of a run: off by at most half a step of
+        the remainder, 2^-22 of the difference, or 2^-21 (half the smallest fp16 step in units of 16).  Runs may span intervals, so differences
+        count from any interval's start.  Replays in 32 bits are off by at most 8 roundings of the largest value a token.  A weight is off by
+        half a step of fp16, 2^-11; as the denominator adds up the rounded weights, that moves the result by no more than twice that of the
+        values' mean distance from it.  The result itself is rounded by half a step."""
         (kp, kz, ko, kn), (vp, vz, vo, vn) = self.values()
         G = self.Hq // self.Hkv
         q = self.q.double().cpu().view(self.B, self.Hkv, G, D)
@@ -131,19 +132,16 @@ class Shared:
             logits = torch.einsum("hgd,htd->hgt", q[b], k) * scaling
             p = torch.softmax(logits, -1)
             o = p @ v
-            sigma = torch.zeros_like(logits)
-            half = torch.maximum(kd * 2.0 ** -11, torch.full_like(kd, 2.0 ** -21))
-            sigma[..., :self.P] = abs(scaling) / math.sqrt(3) * torch.sqrt(torch.einsum("hgd,htd->hgt", q[b] ** 2, half ** 2))
-            # sums of D products in 32 bits (towards zero on the tensor cores), replay
-            sigma = 8 * sigma + abs(scaling) * (D * 2.0 ** -23 + drift) * torch.einsum("hgd,htd->hgt", q[b].abs(), k.abs().amax(1, keepdim=True).expand_as(k))
-            e = sigma.amax(-1, keepdim=True)
-            spread = torch.einsum("hgt,htd->hgd", p, v.abs()) + o.abs()
-            vround = torch.zeros_like(v)
-            vround[:, :self.P] = torch.maximum(vd * 2.0 ** -11, torch.full_like(vd, 2.0 ** -21))
-            wround = torch.zeros_like(v)
-            wround[:, :self.P] = vd * 2.0 ** -11
+            # a logit: the values' roundings, sums of D products in 32 bits (towards zero on the tensor cores), replay
+            off = torch.zeros_like(k)
+            off[:, :self.P] = torch.maximum(kd * 2.0 ** -22, torch.full_like(kd, 2.0 ** -21))
+            off = off + (D * 2.0 ** -23 + drift) * k.abs().amax(1, keepdim=True)
+            e = abs(scaling) * torch.einsum("hgd,htd->hgt", q[b].abs(), off).amax(-1, keepdim=True)
+            away = torch.einsum("hgt,hgtd->hgd", p, (v[:, None] - o[:, :, None]).abs())
+            voff = torch.zeros_like(v)
+            voff[:, :self.P] = torch.maximum(vd * 2.0 ** -22, torch.full_like(vd, 2.0 ** -21))
             out[b] = o
-            bound[b] = torch.expm1(2 * e) * spread + p @ (vround + wround) + (k.shape[1] * 2.0 ** -23 + drift) * (spread + v.abs().amax(1)[:, None]) + \
+            bound[b] = (torch.expm1(2 * e) + 2 * 2.0 ** -11) * away + p @ voff + (k.shape[1] * 2.0 ** -23 + drift) * v.abs().amax(1)[:, None] + \
                 o.abs() * 2.0 ** -11 + 2.0 ** -25
         return out.view(self.B, self.Hq, D), bound.view(self.B, self.Hq, D)
 
