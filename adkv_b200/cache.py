@@ -20,6 +20,9 @@ reference's three calls:
   (``llama_adkv.py:104-123``: O(T^2) bytes moved over a generation); here the buffers are sized for
   ``capacity_tokens`` when the caller knows it, and otherwise doubled -- one copy per doubling, of the used
   words only.
+* **A shared beginning.**  ``fork(batch)`` gives a layer of ``batch`` sequences that go on behind this one-sequence layer: its packed
+  tokens are kept once and replayed once per step for all of them (``gemv.decode_attn_prefix``); the reference would need a copy of the
+  cache per sequence.
 * Options the reference does not have: grouped-query attention (``llama_adkv.py:235-238`` raises), ``bits`` 2,
   ``half_state`` (the fp16-state arithmetic of the reference's CUDA kernels, ``src/adkv/kernel/gemv.cu:150-164``,
   for caches exchanged with them), ``checkpoint_interval`` (recurrence-state checkpoints every that many tokens,
@@ -52,15 +55,16 @@ class KVCacheLayer:
         self._k_tail = self._v_tail = None    # float32 [B, H, 2, D]: state after the last cached token
         self._k_ckpt = self._v_ckpt = None    # float32 [B, H, n, 2, D]: state before token (i+1)*interval
         self._scratch = None
-        self._n = 0                           # cached tokens
+        self._prefix = None                   # gemv.SharedPrefix in front of the cached tokens (see fork)
+        self._n = 0                           # cached tokens, those of a shared prefix not counted
 
     # ------------------------------------------------------------------ what the attention module and HF ask
     def get_seq_length(self) -> int:
-        return self._n
+        return self._n + (self._prefix.tokens if self._prefix else 0)
 
     def get_mask_sizes(self, cache_position) -> tuple[int, int]:
         new = cache_position if isinstance(cache_position, int) else cache_position.shape[0]
-        return self._n + new, 0
+        return self.get_seq_length() + new, 0
 
     @property
     def key_states(self):
@@ -137,6 +141,29 @@ class KVCacheLayer:
                 kw.update(scratch=self._scratch)
         return kw
 
+    # ------------------------------------------------------------------ several sequences behind one
+    def fork(self, batch: int, capacity_tokens: int | None = None) -> "KVCacheLayer":
+        """A layer of ``batch`` sequences whose first tokens are those cached here (one sequence, fused, with tail states, head dim 128).
+
+        The tokens are shared, not copied: they are quantised already, and this layer's buffers are kept alive and read by every step of
+        the new one.  This layer may be continued on its own, and forked again.  With ``checkpoint_interval`` the shared tokens are replayed
+        in parallel runs; without, in one piece per head.  ``capacity_tokens``: own tokens to make room for."""
+        if batch < 1:
+            raise ValueError("a fork needs at least one sequence")
+        if self._prefix is not None:
+            raise ValueError("a layer behind a shared prefix cannot be forked again")
+        if self._geom is None or self._n == 0:
+            raise ValueError("nothing is cached yet that could be shared")
+        B, H, D, device = self._geom
+        if B != 1 or D != 128 or not self._keeps_tails:
+            raise ValueError("only a layer of one sequence with tail states and head dim 128 can be shared")
+        child = KVCacheLayer(bits=self.bits, fast=self.fast, capacity_tokens=capacity_tokens)
+        child._prefix = gemv.SharedPrefix(self._k, self._v, self._n, k_tail=self._k_tail.clone(), v_tail=self._v_tail.clone(), bits=self.bits,
+                                          k_ckpt=self._k_ckpt, v_ckpt=self._v_ckpt, ckpt_interval=self._interval)
+        child._geom = (batch, H, D, device)
+        child._k_tail, child._v_tail = child._prefix.start_tails(batch)
+        return child
+
     @staticmethod
     def _per_head(params, H: int, D: int):
         return tuple(t.view(H, D) for t in params)
@@ -161,7 +188,7 @@ class KVCacheLayer:
         vp = self._per_head((value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target), H, D)
         gemv.encode_kv_pair(self._k, key_states.to(torch.float16), kp, self._v, value_states.to(torch.float16), vp,
                             SCALE_MIN, SCALE_MAX, bits=self.bits, t_start=self._n, half_state=self.half_state,
-                            **self._state_kwargs())
+                            from_tail=self._prefix is not None, **self._state_kwargs())
         self._n += T
 
     # ------------------------------------------------------------------ decode
@@ -188,6 +215,16 @@ class KVCacheLayer:
         mask = attention_mask
         if mask is not None and mask.dim() == 4:
             mask = mask[:, :, 0, :]
+        if self._prefix is not None:
+            if mask is not None:
+                raise ValueError("a layer behind a shared prefix takes no mask")
+            need = gemv.prefix_scratch_bytes(B, Hq, self._prefix)
+            if self._scratch is None or self._scratch.numel() < need:
+                self._scratch = torch.empty(need, dtype=torch.uint8, device=self._geom[3])
+            out = gemv.decode_attn_prefix(q, self._prefix, self._k, self._v, k, v, kp, vp, T, scaling, SCALE_MIN, SCALE_MAX, k_tail=self._k_tail,
+                                          v_tail=self._v_tail, scratch=self._scratch)
+            self._n = T + 1
+            return out.to(query_states.dtype), None
         shared_mask = mask is None or mask.numel() == B * (T + 1)
         if self._interval and not shared_mask:
             raise ValueError("a checkpointed cache takes masks shared by all heads only")
@@ -217,6 +254,12 @@ class KVCache(list):
 
     def __init__(self, num_layers: int, **layer_kwargs):
         super().__init__(KVCacheLayer(**layer_kwargs) for _ in range(num_layers))
+
+    def fork(self, batch: int, capacity_tokens: int | None = None) -> "KVCache":
+        """The caches of ``batch`` sequences that go on behind this one (see :meth:`KVCacheLayer.fork`)."""
+        child = KVCache(0)
+        child.extend(layer.fork(batch, capacity_tokens) for layer in self)
+        return child
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         return self[layer_idx].get_seq_length()

@@ -12,10 +12,13 @@ last token is kept per layer (tail states), so every appended code comes from it
 of the cache runs in the cheaper contracted arithmetic; and the model can be
 tensor-parallel over the GPUs of a node (heads and FFN columns sharded, two NCCL all-reduces per
 layer on the ``[B, d_model]`` activations, which are the only NVLink traffic -- attention itself
-never leaves its GPU).
+never leaves its GPU); queries, keys and values leave the projection through one kernel that
+rotates them (and normalises them per head, ``qk_norm``) into the layout of the caches; several
+completions of one prompt can share its packed cache (``prefill_shared``), and the next token can be
+chosen under penalties, biases and masks (``logit_rules``).
 
-Everything except attention and quantisation is plain torch (cuBLAS GEMMs): it is plumbing around
-the kernels, not part of what is measured against the roofline.
+The rest is plain torch (cuBLAS GEMMs): it is plumbing around the kernels, not part of what is
+measured against the roofline.
 """
 from __future__ import annotations
 
@@ -30,7 +33,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from . import gemv, synth
+from . import gemv, step, synth
 
 
 @dataclass
@@ -44,6 +47,7 @@ class LlamaShape:
     vocab: int = 32000
     rope_theta: float = 10000.0
     norm_eps: float = 1e-5
+    qk_norm: bool = False       # queries and keys are normalised per head before the rotation
 
 
 def _rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -72,8 +76,13 @@ class ADKVLlama:
     def __init__(self, shape: LlamaShape, batch: int, max_tokens: int, bits: int = 4, device="cuda",
                  rank: int = 0, world: int = 1, seed: int = 0, fused: bool = True, fast: bool | None = None,
                  ckpt_interval: int = 0, half_state: bool = False, peers: list | None = None,
-                 split_channels: bool | None = None):
-        """``fast``: None = contracted replay wherever tail states keep the stored codes exact (the fused step in the
+                 split_channels: bool | None = None, shared_tokens: int = 0, shared_interval: int = 128, logit_rules: dict | None = None):
+        """``shared_tokens``: room for a prompt that all sequences share (:meth:`prefill_shared`; fused, fp32 arithmetic, head dim 128, no
+        ``ckpt_interval``), kept once and with state checkpoints every ``shared_interval`` tokens; ``max_tokens`` are then each sequence's
+        own.  ``logit_rules``: arguments of :func:`step.process_logits` for the choice of every next token (``repetition``, ``presence``,
+        ``frequency``, ``bias``, ``mask``); the history they look at is the tokens a sequence was given and has generated.
+
+        ``fast``: None = contracted replay wherever tail states keep the stored codes exact (the fused step in the
         fp32 arithmetic), canonical replay otherwise.  ``peers``: the other tensor-parallel shards when all of them
         live in this process (tests on one GPU); the all-reduce is then a sum over the shards' partial results, and
         the shards are stepped together with :func:`step_together`."""
@@ -86,6 +95,9 @@ class ADKVLlama:
         self.peers = peers
         self.split_channels = split_channels      # layout of a head over warps in the eager fused step (None: automatic)
         self._marks = None                        # event recorder of profile_decode_step
+        self.shared_tokens, self.shared, self.n_shared = shared_tokens, None, 0
+        if shared_tokens and (not self.keeps_tails or ckpt_interval or shape.head_dim != 128):
+            raise ValueError("a shared prompt needs the fused step with tail states, head dim 128 and no ckpt_interval")
         self.hq, self.hkv, self.ffn = shape.n_heads // world, shape.n_kv_heads // world, shape.ffn // world
         D, dm = shape.head_dim, shape.d_model
         g = torch.Generator(device=self.dev)
@@ -133,7 +145,23 @@ class ADKVLlama:
             if ckpt_interval:
                 L["kck"] = gemv.alloc_ckpt(batch, self.hkv, D, max_tokens, ckpt_interval, self.dev)
                 L["vck"] = gemv.alloc_ckpt(batch, self.hkv, D, max_tokens, ckpt_interval, self.dev)
-        self.cos, self.sin = _rope_tables(shape, max_tokens, self.dev)
+        self.cos, self.sin = _rope_tables(shape, shared_tokens + max_tokens, self.dev)
+        if shape.qk_norm:
+            for L in self.layers:
+                L["q_norm"], L["k_norm"] = (torch.ones(D, dtype=torch.float16, device=self.dev) for _ in range(2))
+        self.logit_rules = logit_rules
+        if logit_rules is not None:
+            self.history = torch.zeros((batch, shared_tokens + max_tokens + 1), dtype=torch.int32, device=self.dev)
+            self.history_lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)
+        if shared_tokens:
+            self.shared_scratch = None
+            n = gemv.n_super_for(shared_tokens, bits)
+            for L in self.layers:
+                L["skc"] = torch.zeros((1, self.hkv, n, D // 4, 4, 4), dtype=torch.uint8, device=self.dev)
+                L["svc"] = torch.zeros_like(L["skc"])
+                L["skt"], L["svt"] = (torch.zeros((1, self.hkv, 2, D), dtype=torch.float32, device=self.dev) for _ in range(2))
+                L["sck"], L["scv"] = (gemv.alloc_ckpt(1, self.hkv, D, shared_tokens, shared_interval, self.dev) for _ in range(2))
+            self.shared_interval = shared_interval
         self.T = 0
         self.scaling = D ** -0.5
         self.scratch = None
@@ -167,11 +195,22 @@ class ADKVLlama:
         gate, up = gu[..., :self.ffn], gu[..., self.ffn:]
         return self._allreduce((F.silu(gate) * up) @ L["w_down"].T)
 
-    def _qkv(self, L, h, T_new):
-        B = h.shape[0]
-        D = self.s.head_dim
-        qkv = (h @ L["wqkv"].T).view(B, T_new, self.hq + 2 * self.hkv, D).transpose(1, 2)     # [B, H*, T, D]
-        return qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv], qkv[:, self.hq + self.hkv:]
+    def _qkv(self, L, h, start: int = 0, positions=None):
+        """Rotated queries and keys, and values, ``[B, H*, T, D]``: token t of h at position ``start + t``, or ``positions[b] + t``."""
+        half = self.s.head_dim // 2
+        return step.norm_rope_qkv(h @ L["wqkv"].T, self.hq, self.hkv, self.cos[:, :half], self.sin[:, :half], start=start, positions=positions,
+                                  q_weight=L.get("q_norm"), k_weight=L.get("k_norm"), eps=self.s.norm_eps)
+
+    def _remember(self, tokens: torch.Tensor) -> None:
+        """Add one token per sequence to the history that ``logit_rules`` look at."""
+        if self.logit_rules is not None:
+            self.history.scatter_(1, self.history_lens.long()[:, None], tokens.int()[:, None])
+            self.history_lens += 1
+
+    def _choose(self, logits: torch.Tensor) -> torch.Tensor:
+        if self.logit_rules is None:
+            return logits.argmax(-1)
+        return step.process_logits(logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[1].long()
 
     def _ck(self, L):
         return dict(k_ckpt=L["kck"], v_ckpt=L["vck"], ckpt_interval=self.ckpt_interval) if self.ckpt_interval else {}
@@ -181,17 +220,14 @@ class ADKVLlama:
     def prefill(self, ids: torch.Tensor, batch_chunk: int = 16) -> torch.Tensor:
         """ids [B, Tp] -> next-token ids [B]; fills the caches with the quantised prompt."""
         B, Tp = ids.shape
-        assert B == self.B and self.T == 0
-        cos, sin = self.cos[:Tp], self.sin[:Tp]
+        assert B == self.B and self.T == 0 and not self.shared_tokens
         logits = []
         for b0 in range(0, B, batch_chunk):
             b1 = min(B, b0 + batch_chunk)
             x = self.embed[ids[b0:b1]]
             for L in self.layers:
-                h = _rms_norm(x, L["norm1"], self.s.norm_eps)
-                q, k, v = self._qkv(L, h, Tp)
-                q, k = _apply_rope(q, cos, sin), _apply_rope(k, cos, sin)
-                gemv.encode_kv_pair(L["kc"][b0:b1], k.contiguous(), L["kp"], L["vc"][b0:b1], v.contiguous(), L["vp"],
+                q, k, v = self._qkv(L, _rms_norm(x, L["norm1"], self.s.norm_eps))
+                gemv.encode_kv_pair(L["kc"][b0:b1], k, L["kp"], L["vc"][b0:b1], v, L["vp"],
                                     synth.SCALE_MIN, synth.SCALE_MAX, bits=self.bits, half_state=self.half_state,
                                     **self._tails(L, b0, b1),
                                     **({"k_ckpt": L["kck"][b0:b1], "v_ckpt": L["vck"][b0:b1],
@@ -203,18 +239,54 @@ class ADKVLlama:
             logits.append(last @ self.lm_head.T)
         self.T = Tp
         self.last_logits = torch.cat(logits)
-        return self.last_logits.argmax(-1)
+        if self.logit_rules is not None:
+            self.history[:, :Tp] = ids
+            self.history_lens.fill_(Tp)
+        return self._choose(self.last_logits)
+
+    @torch.no_grad()
+    def prefill_shared(self, ids: torch.Tensor) -> torch.Tensor:
+        """ids [P]: the prompt that all sequences share, prefilled once -> their first tokens [B], the most likely ones in turn (the same
+        for all would be the same completion)."""
+        P = ids.numel()
+        assert ids.dim() == 1 and 0 < P <= self.shared_tokens and self.T == 0 and self.shared is None
+        x = self.embed[ids][None]
+        prefixes = []
+        for L in self.layers:
+            q, k, v = self._qkv(L, _rms_norm(x, L["norm1"], self.s.norm_eps))
+            ck = dict(k_ckpt=L["sck"], v_ckpt=L["scv"], ckpt_interval=self.shared_interval)
+            gemv.encode_kv_pair(L["skc"], k, L["kp"], L["svc"], v, L["vp"], synth.SCALE_MIN, synth.SCALE_MAX, bits=self.bits, k_tail=L["skt"],
+                                v_tail=L["svt"], **ck)
+            prefixes.append(gemv.SharedPrefix(L["skc"], L["svc"], P, k_tail=L["skt"], v_tail=L["svt"], bits=self.bits, **ck))
+            for t, tail in zip((L["kt"], L["vt"]), prefixes[-1].start_tails(self.B)):
+                t.copy_(tail)
+            att = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.hq != self.hkv)
+            x = x + self._allreduce(att.transpose(1, 2).reshape(1, P, -1) @ L["wo"].T)
+            x = x + self._mlp(L, _rms_norm(x, L["norm2"], self.s.norm_eps))
+        self.shared, self.n_shared = prefixes, P
+        for L, prefix in zip(self.layers, prefixes):
+            L["shared"] = prefix
+        self.shared_scratch = torch.empty(gemv.prefix_scratch_bytes(self.B, self.hq, prefixes[0]), dtype=torch.uint8, device=self.dev)
+        self.last_logits = (_rms_norm(x[:, -1], self.final_norm, self.s.norm_eps) @ self.lm_head.T).expand(self.B, -1)
+        if self.logit_rules is not None:
+            self.history[:, :P] = ids
+            self.history_lens.fill_(P)
+            logits = step.process_logits(self.last_logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[0]
+            return logits.float().topk(self.B, -1).indices.diagonal()
+        return self.last_logits[0].float().topk(self.B).indices
 
     # ------------------------------------------------------------------ the two halves of a layer, before the all-reduce
-    def _attn_partial(self, L, x, T, cos, sin, seq_lens=None):
-        """This shard's part of the attention block's output for one new token per sequence: [B, 1, d_model]."""
+    def _attn_partial(self, L, x, T, seq_lens=None, positions=None):
+        """This shard's part of the attention block's output for one new token per sequence: [B, 1, d_model].  T own tokens are cached;
+        with ``seq_lens`` their number is on the device, and ``positions`` holds where the new tokens are."""
         h = _rms_norm(x, L["norm1"], self.s.norm_eps)
-        q, k, v = self._qkv(L, h, 1)
-        q, k = _apply_rope(q, cos, sin).contiguous(), _apply_rope(k, cos, sin).contiguous()
-        v = v.contiguous()
+        q, k, v = self._qkv(L, h, 0 if positions is not None else self.n_shared + T, positions)
         self._mark("norm_qkv_rope")
         smin, smax = synth.SCALE_MIN, synth.SCALE_MAX
-        if seq_lens is not None:
+        if self.n_shared:
+            att = gemv.decode_attn_prefix(q, L["shared"], L["kc"], L["vc"], k, v, L["kp"], L["vp"], T if seq_lens is None else seq_lens, self.scaling,
+                                          smin, smax, scratch=self.shared_scratch, **self._tails(L))
+        elif seq_lens is not None:
             att = gemv.decode_attn_varlen(q, L["kc"], L["vc"], k, v, L["kp"], L["vp"], seq_lens, self.scaling, smin, smax,
                                           bits=self.bits, fast=self.fast, half_state=self.half_state, **self._tails(L))
         elif self.fused:
@@ -241,7 +313,7 @@ class ADKVLlama:
     def _head(self, x):
         last = _rms_norm(x[:, 0], self.final_norm, self.s.norm_eps)
         self.last_logits = last @ self.lm_head.T
-        tok = self.last_logits.argmax(-1)
+        tok = self._choose(self.last_logits)
         self._mark("final_norm_lm_head")
         return tok
 
@@ -273,11 +345,11 @@ class ADKVLlama:
         """One decode step in which nothing on the host depends on the position: the token count lives in
         ``self.seq_lens`` on the device (read by the attention kernel and the RoPE lookup, incremented at the
         end), so the recorded sequence of launches is the same for every step."""
-        pos = self.seq_lens[:1].long()
-        cos, sin = self.cos.index_select(0, pos), self.sin.index_select(0, pos)
+        self._remember(ids)
+        positions = self.seq_lens + self.n_shared if self.n_shared else self.seq_lens
         x = self.embed[ids][:, None, :]
         for L in self.layers:
-            x = x + self._allreduce(self._attn_partial(L, x, None, cos, sin, seq_lens=self.seq_lens))
+            x = x + self._allreduce(self._attn_partial(L, x, None, seq_lens=self.seq_lens, positions=positions))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.seq_lens += 1
         return self._head(x)
@@ -319,10 +391,10 @@ class ADKVLlama:
     def decode(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B] (the tokens at position T) -> next-token ids [B]; appends position T to the caches."""
         T = self.T
-        cos, sin = self.cos[T:T + 1], self.sin[T:T + 1]
+        self._remember(ids)
         x = self.embed[ids][:, None, :]                                                  # [B, 1, dm]
         for L in self.layers:
-            x = x + self._allreduce(self._attn_partial(L, x, T, cos, sin))
+            x = x + self._allreduce(self._attn_partial(L, x, T))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.T = T + 1
         return self._head(x)
@@ -334,10 +406,9 @@ def step_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
     :meth:`ADKVLlama.decode`, with each all-reduce replaced by the sum of the shards' partial results.  Used to
     test the sharding (head slices of weights and ADKV parameters, caches per shard) without several GPUs."""
     T = shards[0].T
-    cos, sin = shards[0].cos[T:T + 1], shards[0].sin[T:T + 1]
     x = shards[0].embed[ids][:, None, :]
     for li in range(len(shards[0].layers)):
-        x = x + torch.stack([m._attn_partial(m.layers[li], x, T, cos, sin) for m in shards]).sum(0)
+        x = x + torch.stack([m._attn_partial(m.layers[li], x, T) for m in shards]).sum(0)
         x = x + torch.stack([m._mlp_partial(m.layers[li], x) for m in shards]).sum(0)
     for m in shards:
         m.T = T + 1
@@ -351,15 +422,13 @@ def step_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
 def prefill_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
     """Prefill of co-resident shards (see :func:`step_together`)."""
     B, Tp = ids.shape
-    cos, sin = shards[0].cos[:Tp], shards[0].sin[:Tp]
     x = shards[0].embed[ids]
     for li in range(len(shards[0].layers)):
         parts = []
         for m in shards:
             L = m.layers[li]
-            q, k, v = m._qkv(L, _rms_norm(x, L["norm1"], m.s.norm_eps), Tp)
-            q, k = _apply_rope(q, cos, sin), _apply_rope(k, cos, sin)
-            gemv.encode_kv_pair(L["kc"], k.contiguous(), L["kp"], L["vc"], v.contiguous(), L["vp"], synth.SCALE_MIN,
+            q, k, v = m._qkv(L, _rms_norm(x, L["norm1"], m.s.norm_eps))
+            gemv.encode_kv_pair(L["kc"], k, L["kp"], L["vc"], v, L["vp"], synth.SCALE_MIN,
                                 synth.SCALE_MAX, bits=m.bits, half_state=m.half_state, **m._tails(L))
             att = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=m.hq != m.hkv)
             parts.append(att.transpose(1, 2).reshape(B, Tp, -1) @ L["wo"].T)
@@ -371,8 +440,10 @@ def prefill_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
 
 
 def run(shape: LlamaShape, batch: int, prompt: int, gen: int, bits: int = 4, fused: bool = True, fast: bool | None = None,
-        ckpt_interval: int = 0, seed: int = 0, graph: bool = False, half_state: bool = False, breakdown: int = 0) -> dict:
-    """Prefill a random prompt, generate `gen` tokens greedily; timings with CUDA events, max over ranks."""
+        ckpt_interval: int = 0, seed: int = 0, graph: bool = False, half_state: bool = False, breakdown: int = 0,
+        shared_prompt: bool = False, logit_rules: dict | None = None) -> dict:
+    """Prefill a random prompt, generate `gen` tokens greedily; timings with CUDA events, max over ranks.  ``shared_prompt``: one prompt for
+    all sequences, kept once; ``logit_rules`` as in :class:`ADKVLlama`."""
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
     local = int(os.environ.get("LOCAL_RANK", "0"))
@@ -380,8 +451,9 @@ def run(shape: LlamaShape, batch: int, prompt: int, gen: int, bits: int = 4, fus
     dev = torch.device("cuda", local)
     if world > 1 and not dist.is_initialized():
         dist.init_process_group("nccl", device_id=dev)
-    model = ADKVLlama(shape, batch, prompt + gen + breakdown, bits=bits, device=dev, rank=rank, world=world, seed=seed,
-                      fused=fused, fast=fast, ckpt_interval=ckpt_interval, half_state=half_state)
+    model = ADKVLlama(shape, batch, (0 if shared_prompt else prompt) + gen + breakdown, bits=bits, device=dev, rank=rank, world=world, seed=seed,
+                      fused=fused, fast=fast, ckpt_interval=ckpt_interval, half_state=half_state,
+                      shared_tokens=prompt if shared_prompt else 0, logit_rules=logit_rules)
     g = torch.Generator(device=dev)
     g.manual_seed(seed + 99)
     ids = torch.randint(0, shape.vocab, (batch, prompt), generator=g, device=dev)
@@ -390,7 +462,7 @@ def run(shape: LlamaShape, batch: int, prompt: int, gen: int, bits: int = 4, fus
         dist.barrier()
     torch.cuda.synchronize(dev)
     ev[0].record()
-    tok = model.prefill(ids)
+    tok = model.prefill_shared(ids[0]) if shared_prompt else model.prefill(ids)
     ev[1].record()
     out = [tok]
     if graph:
@@ -408,7 +480,7 @@ def run(shape: LlamaShape, batch: int, prompt: int, gen: int, bits: int = 4, fus
     ev[2].record()
     torch.cuda.synchronize(dev)
     step_breakdown = None
-    if breakdown and model.T + breakdown <= prompt + gen + breakdown:
+    if breakdown:
         # extra eager steps after the timed region (the caches were sized for them)
         _, step_breakdown = model.profile_decode_step(tok, breakdown)
     t = torch.tensor([ev[0].elapsed_time(ev[1]), ev[1].elapsed_time(ev[2])], dtype=torch.float64, device=dev)
@@ -419,7 +491,7 @@ def run(shape: LlamaShape, batch: int, prompt: int, gen: int, bits: int = 4, fus
     toks = torch.stack(out, 1)
     return dict(rank=rank, world=world, prefill_ms=prefill_ms, decode_ms=decode_ms,
                 decode_tokens_per_s=batch * gen / (decode_ms * 1e-3), ms_per_decode_step=decode_ms / gen,
-                prefill_tokens_per_s=batch * prompt / (prefill_ms * 1e-3), device_status=status,
+                prefill_tokens_per_s=(1 if shared_prompt else batch) * prompt / (prefill_ms * 1e-3), device_status=status,
                 token_checksum=int(toks.sum().item()), tokens=toks, fast=bool(model.fast),
                 tail_states=model.keeps_tails, eager_step_breakdown_ms=step_breakdown)
 
@@ -438,6 +510,8 @@ def main():
                     help="the fp16-state arithmetic of the reference's CUDA kernels instead of the fp32 recurrence")
     ap.add_argument("--ckpt-interval", type=int, default=0)
     ap.add_argument("--graph", action="store_true", help="replay the decode step from a CUDA graph (device-side lengths)")
+    ap.add_argument("--shared-prompt", action="store_true", help="all sequences complete one prompt, whose packed cache is kept once")
+    ap.add_argument("--repetition", type=float, default=1.0, help="penalty on tokens that a sequence holds already")
     ap.add_argument("--breakdown", type=int, default=0,
                     help="after the timed run, this many extra eager steps with CUDA events around every segment "
                          "(attention kernels, projections, MLP, all-reduces)")
@@ -445,14 +519,15 @@ def main():
     shape = LlamaShape(n_layers=a.layers)
     r = run(shape, a.batch, a.prompt, a.gen, bits=a.bits, fused=not a.unfused,
             fast=True if a.fast else (False if a.exact else None),
-            ckpt_interval=a.ckpt_interval, graph=a.graph, half_state=a.half_state, breakdown=a.breakdown)
+            ckpt_interval=a.ckpt_interval, graph=a.graph, half_state=a.half_state, breakdown=a.breakdown,
+            shared_prompt=a.shared_prompt, logit_rules=dict(repetition=a.repetition) if a.repetition != 1.0 else None)
     if r["rank"] == 0:
         r.pop("tokens")
         r.update(metric="e2e_decode_tokens_per_s", config=dict(model="random-init Llama-2-7B architecture", batch=a.batch,
                  prompt=a.prompt, generate=a.gen, layers=a.layers, bits=a.bits, fused=not a.unfused,
                  replay="half" if a.half_state else ("contracted" if r["fast"] else "canonical"),
                  tail_states=r["tail_states"], tensor_parallel=r["world"],
-                 cuda_graph=a.graph, data="synthetic"))
+                 cuda_graph=a.graph, shared_prompt=a.shared_prompt, repetition=a.repetition, data="synthetic"))
         print(json.dumps(r), flush=True)
     if dist.is_initialized():
         dist.barrier()
