@@ -6,17 +6,22 @@
 // With x the replayed keys and y the replayed values of one KV head, the prefix part of all R = B * Hq / Hkv query rows is
 //   S = Q x^T,  P = exp2(S * scaling * log2(e) - m),  O = P y,  l = sum P
 // two products of matrices around a recurrence that serves every row, so the recurrence stays on the SIMT side, a channel a thread, and
-// the products go to tcgen05: 128 query rows by 64 tokens at a time, Q and the replayed tiles in shared memory, S, P and O in tensor
+// the products go to tcgen05: 128 query rows by 32 tokens at a time, the replayed tiles in shared memory, Q, S, P and O in tensor
 // memory.  A CTA takes 128 rows of one head and a run of checkpoint intervals (state checkpoints make runs independent), leaves maximum,
-// denominator and sums of each row in scratch memory, and the merge of adkv_split.cu joins them with the sequences' own parts.
+// denominator and sums of each row in scratch memory, and a join adds the runs up with the sequences' own parts.
 //
 // Values are fp16 numbers for the products, as differences from the zero point at the start of the run: that point's share of a logit is
 // the same for the whole run and is added in fp32 to the maximum, its share of the result to the sums, so a channel far from zero keeps the
 // bits of its deviations.  They are held in units of 16, a power of two, so that differences up to a million are in range.  One fp16 number
 // is 2^-11 of a value: with channels that reach 50, as the outliers of this library's benchmark do, logits would be off by some 1e-3 and
-// results by up to 2.7 times what its results may be off (2e-3 and 2e-3 of the value), so K and V are pairs, rounded value and remainder
-// (22 bits), for two more products.  Weights are rounded to fp16, and the denominator adds them up as rounded, so that what a weight is
-// off cancels where it dominates; sums of all products are fp32.
+// results by up to 2.7 times what its results may be off (2e-3 and 2e-3 of the value); with weights of 11 bits it would be up to 1.2 times.
+// So K, V and the weights are pairs, rounded number and remainder (22 bits), for three more products, and sums are fp32: what is left are
+// the fp16 queries and results that every step of the library has.  The pairs of the weights cost 1 % (64 sequences 69.4 -> 70.4 us).
+//
+// 8192 tokens of 32 heads, 4-bit: 58 us for 4 sequences, 70 us for 64, 85 us for 128; 16000 of 8 heads, 2-bit, 47 us for 32 x 4.  The bytes
+// would take 5 us.  The scans bound it: 256 recurrences of some 20 instructions a token and head, 10.2 cycles a value and scheduler in a
+// bare loop, here a third more for waits among the warps, and a sixth of the time is filling and emptying (first words 2 us, results 3 us).
+// Tiles of 64 tokens, worked on in halves: within 3 % of that, but 15.2 instead of 14.0 us where the prefix has 300 tokens.
 #include "adkv_host.h"
 
 #include <algorithm>
@@ -26,7 +31,8 @@
 
 namespace adkv {
 
-constexpr int kPreTok = 64, kPreRows = 128;   // tokens of a tile, query rows of a CTA
+constexpr int kPreTok = 32, kPreRows = 128;   // tokens of a tile, query rows of a CTA
+constexpr int kPreK = 4, kPreV = 2;           // tiles of K and of V (of S, weights) that are on their way at once
 constexpr int kPreWarps = 14;                 // 0-3: K, 4-7: V (a channel a thread), 8-11: softmax (a row a thread), 12, 13: products
 constexpr int kPreThreads = 32 * kPreWarps;
 constexpr float kPreUnit = 16.f;              // values are held in units of this
@@ -57,20 +63,20 @@ struct PrefixPlan {
 
 template <int BITS>
 struct PrefixShared {
-    alignas(128) __half q[kD / 8][kPreRows][8];          // [channel / 8][row][channel % 8]
-    // K, V; half of a tile: [token / 8][channel][token % 8], the rounded values in the first four rows and the remainders in the others
-    alignas(128) __half x[2][2][kPreTok / 8][kD][8];
-    alignas(128) uint32_t words[2][2][kPreTok * BITS / 32][kD];   // packed tiles of K and V
-    alignas(16) float z0[kD];                            // zero points of K before the run
-    // The results of the run lie in x and what follows, a row every kPartStride floats (no two of eight in the same banks), and the zero
-    // points of V before the run in the last row of words, where only their own thread has read.
-    __device__ float *row(int r) { return reinterpret_cast<float *>(&x[0][0][0][0][0]) + r * kPartStride; }
-    __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][1][kPreTok * BITS / 32 - 1][0]); }
+    // values of a tile: [token / 8][channel][token % 8], the rounded ones in the first half and the remainders in the other
+    alignas(128) __half k[kPreK][2 * kPreTok / 8][kD][8];
+    alignas(128) __half v[kPreV][2 * kPreTok / 8][kD][8];
+    alignas(128) uint32_t words[2][kPreK][kPreTok * BITS / 32][kD];   // packed tiles of K and V
+    alignas(16) float base[kPreRows];                    // what the zero points of K before the run add to every logit of a row
+    // The results of the run lie in k and v, a row every kPartStride floats (no two of eight in the same banks), and the zero points of V
+    // before the run in the last row of words, where only their own thread has read.
+    __device__ float *row(int r) { return reinterpret_cast<float *>(&k[0][0][0][0]) + r * kPartStride; }
+    __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][kPreK - 1][kPreTok * BITS / 32 - 1][0]); }
     uint32_t tmem;
     int dead;                                            // a bounded wait gave up
-    // of tile i, buffer i % 2: words are there; S is there; weights are there; O is added up (and the weights have been read)
-    uint64_t loaded[2][2], sdone[2], pfull[2], odone[2];
-    uint64_t full[2][2], read[2][2];                     // of K and V, halves of a tile: values are there, have been read
+    // of tile i, slot i % kPreK or i % kPreV: words are there; K values are there, have been read; V values are there; S is there; weights
+    // are there; O is added up (and V and the weights have been read)
+    uint64_t loaded[2][kPreK], kfull[kPreK], kread[kPreK], vfull[kPreV], sdone[kPreV], pfull[kPreV], odone[kPreV];
 };
 
 // K-major shared-memory matrix without swizzle: element (m, k) lies at (m / 8) * m_stride + (k / 8) * k_stride + (m % 8) * 16 + (k % 8) * 2.
@@ -92,26 +98,49 @@ template <int BITS, bool GUARDED>
 __device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS> &fc, PrefixChan &c, float smin, float smax, int left, float &least,
                                               float &most, uint8_t *dst)
 {
-    float x[8], s0 = 0.f;
-    static_for<8>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        if (!GUARDED && j == 0) s0 = c.s;
-        if (!GUARDED && j == 4) {
-            least = fminf(fminf(least, s0), c.s);
-            most = fmaxf(fmaxf(most, s0), c.s);
-        }
-        const float q = fc.template code<j % 4>(j < 4 ? w : w >> (4 * BITS));
-        const float rh = __fmul_rn(q, GUARDED ? fmaxf(c.s, kEps / kPreUnit) : c.s);
-        x[j] = __fadd_rn(rh, c.zp);
-        if (GUARDED && j >= left) x[j] = 0.f;   // behind the last token: whatever the words hold there does not count
-        c.zp = fmaf(c.alpha, rh, c.zp);
-        c.s *= fmaf(c.beta, fabsf(q), c.tc);
-        if (GUARDED) c.s = fminf(fmaxf(c.s, smin), smax);
-    });
+    float x[8];
+    if constexpr (GUARDED) {
+        static_for<8>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const float q = fc.template code<j % 4>(j < 4 ? w : w >> (4 * BITS));
+            const float rh = __fmul_rn(q, fmaxf(c.s, kEps / kPreUnit));
+            x[j] = j < left ? __fadd_rn(rh, c.zp) : 0.f;   // behind the last token: whatever the words hold there does not count
+            c.zp = fmaf(c.alpha, rh, c.zp);
+            c.s = fminf(fmaxf(c.s * fmaf(c.beta, fabsf(q), c.tc), smin), smax);
+        });
+    } else {
+        // Codes and scale factors of two tokens at a time: they need no state.  With the other products in pairs, too, register moves and
+        // reads eat up what that saves: 12.1 cycles a value and scheduler one by one, 10.2 like this, 10.9 and 11.3 with more pairs (bare loop).
+        const f32x2 beta2 = pk2(c.beta, c.beta), tc2 = pk2(c.tc, c.tc);
+        float s0 = 0.f;
+        static_for<4>([&](auto jc) {
+            constexpr int j = 2 * decltype(jc)::value, k = j % 4;
+            if (j == 0) s0 = c.s;
+            if (j == 4) {
+                least = fminf(fminf(least, s0), c.s);
+                most = fmaxf(fmaxf(most, s0), c.s);
+            }
+            const uint32_t group = j < 4 ? w : w >> (4 * BITS);
+            uint32_t f0, f1;   // FieldConsts::code of fields k and k + 1, before the constant is taken off
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(f0) : "r"(group), "n"(Codec<BITS>::FIELD << (BITS * k)), "r"(fc.e[k]));
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(f1) : "r"(group), "n"(Codec<BITS>::FIELD << (BITS * (k + 1))), "r"(fc.e[k + 1]));
+            const f32x2 q2 = add2(pk2(__uint_as_float(f0), __uint_as_float(f1)), pk2(__uint_as_float(fc.negc[k]), __uint_as_float(fc.negc[k + 1])));
+            float q[2], f[2];
+            upk2(q2, q[0], q[1]);
+            upk2(fma2(beta2, abs2(q2), tc2), f[0], f[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float rh = __fmul_rn(q[i], c.s);
+                x[j + i] = __fadd_rn(rh, c.zp);
+                c.zp = fmaf(c.alpha, rh, c.zp);
+                c.s *= f[i];
+            }
+        });
+    }
     const uint4 hi = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
     *reinterpret_cast<uint4 *>(dst) = hi;
-    *reinterpret_cast<uint4 *>(dst + (kPreTok / 16) * kD * 16) = make_uint4(pack_remainder(hi.x, x[0], x[1]), pack_remainder(hi.y, x[2], x[3]),
-                                                                            pack_remainder(hi.z, x[4], x[5]), pack_remainder(hi.w, x[6], x[7]));
+    *reinterpret_cast<uint4 *>(dst + (kPreTok / 8) * kD * 16) = make_uint4(pack_remainder(hi.x, x[0], x[1]), pack_remainder(hi.y, x[2], x[3]),
+                                                                           pack_remainder(hi.z, x[4], x[5]), pack_remainder(hi.w, x[6], x[7]));
 }
 
 __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreSlack
@@ -119,12 +148,6 @@ __device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
-}
-// v plus the halves of h
-__device__ __forceinline__ float add_halves(uint32_t h, float v)
-{
-    asm("{.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tadd.rn.f32.f16 %0, x, %0;\n\tadd.rn.f32.f16 %0, y, %0;\n\t}" : "+f"(v) : "r"(h));
-    return v;
 }
 __device__ __forceinline__ void warp_arrive(uint64_t *bar, int lane, int count = 1)
 {
@@ -138,19 +161,16 @@ __device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// The 64 columns of a tile, 16 at a time: the next ones are on their way while use() works on these.
-template <class F>
-__device__ __forceinline__ void for_columns(uint32_t cols, const F &use)
+// a warp's 32 lanes x 32 columns; finished at tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t at)
 {
-    uint32_t v[2][16];
-    tmem_ld(v[0], cols);
-    tmem_wait_ld(v[0]);
-#pragma unroll
-    for (int n = 0; n < kPreTok / 16; ++n) {
-        if (n + 1 < kPreTok / 16) tmem_ld(v[(n + 1) & 1], cols + 16 * (n + 1));
-        use(16 * n, v[n & 1]);
-        if (n + 1 < kPreTok / 16) tmem_wait_ld(v[(n + 1) & 1]);
-    }
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+                 "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+                   "=r"(r[31])
+                 : "r"(at));
 }
 
 template <int BITS>
@@ -159,19 +179,21 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PrefixShared<BITS> &sh = *reinterpret_cast<PrefixShared<BITS> *>(smem_raw);
     constexpr int TPW = Codec<BITS>::TPW, WORDS = kPreTok / TPW;                // word rows of a tile
-    constexpr uint32_t kColS = 0, kColO = 2 * kPreTok, kColumns = 256;          // S (and P in its place) twice, O
+    constexpr uint32_t kColQ = 0, kColS = kD / 2, kColO = kColS + kPreV * kPreTok, kColumns = 256;   // Q; S, with the weights in its place; O
+    static_assert(kColO + kD <= kColumns, "columns of tensor memory");
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hkv;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the sequences' own tokens may be scanned beside this kernel
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kPreK; ++i) {
             mbar_init(&sh.loaded[0][i], 1);
             mbar_init(&sh.loaded[1][i], 1);
-            for (int k = 0; k < 2; ++k) {
-                mbar_init(&sh.full[k][i], 4);
-                mbar_init(&sh.read[k][i], 1);
-            }
+            mbar_init(&sh.kfull[i], 4);
+            mbar_init(&sh.kread[i], 1);
+        }
+        for (int i = 0; i < kPreV; ++i) {
+            mbar_init(&sh.vfull[i], 4);
             mbar_init(&sh.sdone[i], 1);
             mbar_init(&sh.pfull[i], 4);
             mbar_init(&sh.odone[i], 1);
@@ -202,40 +224,10 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         const int rows = min(kPreRows, a.rows - rt * kPreRows);
         // packed tile i of K or V, by one lane of a warp
         const auto load_tile = [&](int tensor, int i) {
-            const int tile = done + i, n = min(WORDS, (ntok + TPW - 1) / TPW - i * WORDS);
-            uint64_t *bar = &sh.loaded[tensor][tile & 1];
+            const int slot = (done + i) % kPreK, n = min(WORDS, (ntok + TPW - 1) / TPW - i * WORDS);
+            uint64_t *bar = &sh.loaded[tensor][slot];
             mbar_expect_tx(bar, n * kD * 4);
-            bulk_load(&sh.words[tensor][tile & 1][0][0], a.cache[tensor] + (size_t(h) * a.n_super_cap + t0 / TPW + size_t(i) * WORDS) * kD * 4,
-                      n * kD * 4, bar);
-        };
-
-        // Query rows, negated where the scaling is negative (rows behind the last one as zeros), by the six warps that are not scanning.
-        const auto load_q = [&](int thread) {
-            const uint32_t sign = a.scaling < 0.f ? 0x80008000u : 0u;
-            constexpr int THREADS = kPreThreads - 256, N = kPreRows * (kD / 8);
-            const auto load = [&](int i) {
-                const int r = i / (kD / 8), k = i % (kD / 8), n = rt * kPreRows + r;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (i < N && r < rows) {
-                    const uint2 *src = reinterpret_cast<const uint2 *>(a.q + (size_t(n >> log_g) * a.Hq + (size_t(h) << log_g) + (n & (G - 1))) * kD + 8 * k);
-                    const uint2 x = src[0], y = src[1];
-                    v = make_uint4(x.x ^ sign, x.y ^ sign, y.x ^ sign, y.y ^ sign);
-                }
-                return v;
-            };
-#pragma unroll 1
-            for (int i = thread; i < N; i += 4 * THREADS) {
-                uint4 v[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = load(i + u * THREADS);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int at = i + u * THREADS;
-                    if (at < N) *reinterpret_cast<uint4 *>(&sh.q[at % (kD / 8)][at / (kD / 8)][0]) = v[u];
-                }
-            }
-            fence_async_shared();
-            asm volatile("bar.sync 1, 192;" ::: "memory");
+            bulk_load(&sh.words[tensor][slot][0][0], a.cache[tensor] + (size_t(h) * a.n_super_cap + t0 / TPW + size_t(i) * WORDS) * kD * 4, n * kD * 4, bar);
         };
 
         if (warp < 8) {
@@ -260,57 +252,51 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             const float lo = gmn > 0.f ? fmaxf(a.smin, kEps) * (1.f / kPreUnit) / (gmn * gmn * gmn * gmn * (1.f - 2e-5f)) : INFINITY;
             const float hi = a.smax * (1.f / kPreUnit) / (gmx * gmx * gmx * gmx * (1.f + 2e-5f));
             PrefixChan ch{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f)};
-            if (which == 0) sh.z0[c] = start;
             bool tame = true;   // no scale of the warp was outside its interval when last looked at
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i) {
-                const int tile = done + i, buf = tile & 1;
-                if (!(ok = mbar_wait(&sh.loaded[which][buf], tile >> 1 & 1, kStatKWait))) break;
-                const uint32_t *row = &sh.words[which][buf][0][c];
-                int left = ntok - i * kPreTok;
-                // Rounds of 32 tokens without guards first, which is right if every fourth scale was inside its interval: one vote a
-                // round.  Where it was not the round is done again with guards, and so are the next ones at once until it is.
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half, left -= kPreTok / 2) {
-                    if (tile >= 1 && !(ok = mbar_wait(&sh.read[which][half], (tile & 1) ^ 1, kStatKWait))) break;
-                    uint8_t *dst = reinterpret_cast<uint8_t *>(&sh.x[which][half][0][c][0]);
-                    uint32_t w[WORDS / 2];
+                const int tile = done + i, slot = tile % kPreK, buf = tile % kPreV;
+                // the words have come, and the products that read this buffer before are done
+                uint64_t *freed = which ? (tile >= kPreV ? &sh.odone[buf] : nullptr) : (tile >= kPreK ? &sh.kread[slot] : nullptr);
+                if (!(ok = mbar_wait_both(&sh.loaded[which][slot], tile / kPreK & 1, freed, (tile / (which ? kPreV : kPreK) & 1) ^ 1, kStatKWait))) break;
+                uint8_t *dst = reinterpret_cast<uint8_t *>(which ? &sh.v[buf][0][c][0] : &sh.k[slot][0][c][0]);
+                const uint32_t *row = &sh.words[which][slot][0][c];
+                const int left = ntok - i * kPreTok;
+                uint32_t w[WORDS];
 #pragma unroll
-                    for (int k = 0; k < WORDS / 2; ++k, row += kD) w[k] = *row;
-                    const float zp = ch.zp, s = ch.s;
-                    bool inside = tame && left >= kPreTok / 2;
-                    if (inside) {
-                        float least = INFINITY, most = -INFINITY;
-                        static_for<kPreTok / 16>([&](auto nc) {
-                            constexpr int n = decltype(nc)::value;
-                            prefix_window<BITS, false>(BITS == 4 ? w[n % (WORDS / 2)] : w[n / 2 % (WORDS / 2)] >> (16 * (n & 1)), fc, ch, 0.f, 0.f, 0, least,
-                                                       most, dst + n * kD * 16);
-                        });
-                        inside = __all_sync(kFull, least >= lo && most <= hi);
-                    }
-                    if (!inside) {
-                        ch.zp = zp;
-                        ch.s = s;
-                        float least = INFINITY, most = -INFINITY;
-#pragma unroll 1
-                        for (int n = 0; n < kPreTok / 16; ++n) {   // rolled: the words move up
-                            least = fminf(least, ch.s);
-                            most = fmaxf(most, ch.s);
-                            prefix_window<BITS, true>(w[0], fc, ch, a.smin * (1.f / kPreUnit), a.smax * (1.f / kPreUnit), left - 8 * n, least, most,
-                                                      dst + n * kD * 16);
-                            if (BITS == 2 && !(n & 1)) {
-                                w[0] >>= 16;
-                            } else {
-#pragma unroll
-                                for (int k = 0; k + 1 < WORDS / 2; ++k) w[k] = w[k + 1];
-                            }
-                        }
-                        tame = __all_sync(kFull, least >= lo && most <= hi);
-                    }
-                    fence_async_shared();
-                    warp_arrive(&sh.full[which][half], lane);
+                for (int k = 0; k < WORDS; ++k) w[k] = row[k * kD];
+                // Without guards first, which is right if every fourth scale was inside its interval: one vote a tile.  Where it was not the
+                // tile is done again with guards, and so are the next ones at once until it is.
+                const float zp = ch.zp, s = ch.s;
+                bool inside = tame && left >= kPreTok;
+                if (inside) {
+                    float least = INFINITY, most = -INFINITY;
+                    static_for<kPreTok / 8>([&](auto nc) {
+                        constexpr int n = decltype(nc)::value;
+                        prefix_window<BITS, false>(BITS == 4 ? w[n % WORDS] : w[n / 2 % WORDS] >> (16 * (n & 1)), fc, ch, 0.f, 0.f, 0, least, most, dst + n * kD * 16);
+                    });
+                    inside = __all_sync(kFull, least >= lo && most <= hi);
                 }
-                if (!ok) break;
+                if (!inside) {
+                    ch.zp = zp;
+                    ch.s = s;
+                    float least = INFINITY, most = -INFINITY;
+#pragma unroll 1
+                    for (int n = 0; n < kPreTok / 8; ++n) {   // rolled: the words move up
+                        least = fminf(least, ch.s);
+                        most = fmaxf(most, ch.s);
+                        prefix_window<BITS, true>(w[0], fc, ch, a.smin * (1.f / kPreUnit), a.smax * (1.f / kPreUnit), left - 8 * n, least, most, dst + n * kD * 16);
+                        if (BITS == 2 && !(n & 1)) {
+                            w[0] >>= 16;
+                        } else {
+#pragma unroll
+                            for (int k = 0; k + 1 < WORDS; ++k) w[k] = w[k + 1];
+                        }
+                    }
+                    tame = __all_sync(kFull, least >= lo && most <= hi);
+                }
+                fence_async_shared();
+                warp_arrive(which ? &sh.vfull[buf] : &sh.kfull[slot], lane);
             }
             if (which == 1) sh.z0_v()[c] = start;
             if (!ok && lane == 0) sh.dead = 1;
@@ -320,78 +306,110 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             const int e = warp & 3, r = 32 * e + lane;
             const bool busy = 32 * e < rows;
             const uint32_t lanes = tmem + (uint32_t(32 * e) << 16);
-            const float f = fabsf(scale2) * kPreUnit;
+            const float f = fmaxf(fabsf(scale2) * kPreUnit, 1e-30f);   // not 0: columns behind the last token are -inf times this
             const int idle = e == 0 ? 4 - (rows + 31) / 32 : 0;        // warps without rows do not take part; the first arrives for them
             float m = -INFINITY, l = 0.f;
-            load_q(threadIdx.x - 256);
+            if (busy) {   // the thread's query row, negated where the scaling is negative (rows behind the last one as zeros)
+                const uint32_t sign = a.scaling < 0.f ? 0x80008000u : 0u;
+                const int n_row = rt * kPreRows + r;
+                const uint2 *src = reinterpret_cast<const uint2 *>(a.q + (size_t(n_row >> log_g) * a.Hq + (size_t(h) << log_g) + (n_row & (G - 1))) * kD);
+                const __half *z_init = a.p[0].zp_init + size_t(h) * kD;
+                const float *z_ckpt = a.ckpt[0] + (size_t(h) * a.n_ckpt_cap + i0 - 1) * 2 * kD;
+                float sum[4] = {};
+#pragma unroll 1
+                for (int n = 0; n < kD / 4; n += 8) {
+                    uint2 v[8];
+                    float4 z[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = r < rows ? src[n + j] : make_uint2(sign, sign);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (i0 > 0) {
+                            z[j] = reinterpret_cast<const float4 *>(z_ckpt)[n + j];
+                        } else {
+                            const uint2 zh = reinterpret_cast<const uint2 *>(z_init)[n + j];
+                            const float2 z0 = __half22float2(*reinterpret_cast<const __half2 *>(&zh.x)), z1 = __half22float2(*reinterpret_cast<const __half2 *>(&zh.y));
+                            z[j] = make_float4(z0.x, z0.y, z1.x, z1.y);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[j].x ^= sign;
+                        v[j].y ^= sign;
+                        const float2 q0 = __half22float2(*reinterpret_cast<const __half2 *>(&v[j].x)), q1 = __half22float2(*reinterpret_cast<const __half2 *>(&v[j].y));
+                        sum[0] = fmaf(q0.x, z[j].x, sum[0]);
+                        sum[1] = fmaf(q0.y, z[j].y, sum[1]);
+                        sum[2] = fmaf(q1.x, z[j].z, sum[2]);
+                        sum[3] = fmaf(q1.y, z[j].w, sum[3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) tmem_st4(lanes + kColQ + 2 * (n + j), v[j].x, v[j].y, v[j + 1].x, v[j + 1].y);
+                }
+                sh.base[r] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+            }
+            asm volatile("bar.sync 1, 160;" ::: "memory");   // with the warp that issues the products
 #pragma unroll 1
             for (int i = 0; i < n_tiles && busy; ++i) {
-                const int tile = done + i, buf = tile & 1;
-                if (!(ok = mbar_wait(&sh.sdone[buf], tile >> 1 & 1, kStatLFullWait))) break;
+                const int tile = done + i, buf = tile % kPreV;
+                if (!(ok = mbar_wait(&sh.sdone[buf], tile / kPreV & 1, kStatLFullWait))) break;
                 tc_fence_after();
                 const uint32_t cols = lanes + kColS + kPreTok * buf;
                 const int left = ntok - i * kPreTok;
-                float top = -INFINITY;
-                const auto largest = [&](auto whole) {
-                    for_columns(cols, [&](int n, const uint32_t (&v)[16]) {
+                uint32_t v[kPreTok];
+                tmem_ld32(v, cols);
+                tmem_wait_ld(v);
+                if (left < kPreTok) {
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float s0 = __uint_as_float(v[j]), s1 = __uint_as_float(v[j + 1]);
-                            if (decltype(whole)::value) top = fmaxf(fmaxf(top, s0), s1);
-                            else top = fmaxf(fmaxf(top, n + j < left ? s0 : -INFINITY), n + j + 1 < left ? s1 : -INFINITY);
-                        }
-                    });
-                };
-                if (left >= kPreTok) largest(std::true_type{});
-                else largest(std::false_type{});
+                    for (int j = 0; j < kPreTok; ++j) v[j] = j < left ? v[j] : 0xff800000u;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < kPreTok; j += 2) top = fmaxf(fmaxf(top, __uint_as_float(v[j])), __uint_as_float(v[j + 1]));
                 top *= f;
                 const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
                 if (__any_sync(kFull, grown)) {
                     const float corr = grown ? exp2_fast(m - top) : 1.f;
                     if (i > 0) {
                         // all sums so far are in: O can be changed
-                        if (!(ok = mbar_wait(&sh.odone[buf ^ 1], (tile - 1) >> 1 & 1, kStatVWait))) break;
+                        if (!(ok = mbar_wait(&sh.odone[(tile - 1) % kPreV], (tile - 1) / kPreV & 1, kStatVWait))) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int n = 0; n < kD; n += 16) {
-                            uint32_t v[16];
-                            tmem_ld(v, lanes + kColO + n);
-                            tmem_wait_ld(v);
+                            uint32_t o[16];
+                            tmem_ld(o, lanes + kColO + n);
+                            tmem_wait_ld(o);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
 #pragma unroll
-                            for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            for (int j = 0; j < 16; j += 4) tmem_st4(lanes + kColO + n + j, o[j], o[j + 1], o[j + 2], o[j + 3]);
                         }
                     }
                     l *= corr;
                     if (grown) m = top;
                 }
-                // the weights take the place of columns that have been read
-                const auto weigh = [&](auto whole) {
-                    for_columns(cols, [&](int n, const uint32_t (&v)[16]) {
-                        uint32_t p[8];
+                float sum[4] = {};
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            float p0 = exp2_fast(fmaf(__uint_as_float(v[j]), f, -m)), p1 = exp2_fast(fmaf(__uint_as_float(v[j + 1]), f, -m));
-                            if (!decltype(whole)::value) {
-                                p0 = n + j < left ? p0 : 0.f;
-                                p1 = n + j + 1 < left ? p1 : 0.f;
-                            }
-                            p[j / 2] = pack_half2(p0, p1);
-                            l = add_halves(p[j / 2], l);   // as they have been rounded: what a weight is off cancels where it dominates
-                        }
-                        tmem_st4(cols + n / 2, p[0], p[1], p[2], p[3]);
-                        tmem_st4(cols + n / 2 + 4, p[4], p[5], p[6], p[7]);
-                    });
-                };
-                if (left >= kPreTok) weigh(std::true_type{});
-                else weigh(std::false_type{});
+                for (int j = 0; j < kPreTok; j += 8) {
+                    uint32_t p[4], rest[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float p0 = exp2_fast(fmaf(__uint_as_float(v[j + 2 * k]), f, -m)), p1 = exp2_fast(fmaf(__uint_as_float(v[j + 2 * k + 1]), f, -m));
+                        p[k] = pack_half2(p0, p1);
+                        rest[k] = pack_remainder(p[k], p0, p1);
+                        sum[k] += p0 + p1;
+                    }
+                    tmem_st4(cols + j / 2, p[0], p[1], p[2], p[3]);
+                    tmem_st4(cols + kPreTok / 2 + j / 2, rest[0], rest[1], rest[2], rest[3]);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 tc_fence_before();
                 warp_arrive(&sh.pfull[buf], lane, 1 + idle);
             }
             const int end = done + n_tiles - 1;
-            if (ok && busy) ok = mbar_wait(&sh.odone[end & 1], end >> 1 & 1, kStatVWait);
+            if (ok && busy) ok = mbar_wait(&sh.odone[end % kPreV], end / kPreV & 1, kStatVWait);
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             const bool dead = sh.dead != 0;
@@ -401,38 +419,25 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                 const int slot = blockIdx.x - plan.first_cta(unit);
                 float *part = a.scratch + ((size_t(n_row >> log_g) * a.Hkv + h) * plan.n_parts + slot) * (kPartStride << log_g) + (n_row & (G - 1)) * kPartStride;
                 float *row = sh.row(r);
-                // what the zero points before the run add to every logit of the row
-                float sum[8] = {};
-#pragma unroll 2
-                for (int k = 0; k < kD / 8; ++k) {
-                    const uint4 q8 = *reinterpret_cast<const uint4 *>(&sh.q[k][r][0]);
-                    const float4 z0 = *reinterpret_cast<const float4 *>(&sh.z0[8 * k]), z1 = *reinterpret_cast<const float4 *>(&sh.z0[8 * k + 4]);
-                    const float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
-                    const uint32_t q2[4] = {q8.x, q8.y, q8.z, q8.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 qf = __half22float2(*reinterpret_cast<const __half2 *>(&q2[j]));
-                        sum[2 * j] = fmaf(qf.x, z[2 * j], sum[2 * j]);
-                        sum[2 * j + 1] = fmaf(qf.y, z[2 * j + 1], sum[2 * j + 1]);
-                    }
-                }
-                const float base = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
                 *reinterpret_cast<float4 *>(row) = dead ? make_float4(-INFINITY, __int_as_float(0x7fc00000), 0.f, 0.f)
-                                                        : make_float4(fmaf(base, fabsf(scale2), m), l, 0.f, 0.f);
+                                                        : make_float4(fmaf(sh.base[r], fabsf(scale2), m), l, 0.f, 0.f);
 #pragma unroll 1
                 for (int n = 0; n < kD; n += 32) {
-                    uint32_t v[2][16];
-                    tmem_ld(v[0], lanes + kColO + n);
-                    tmem_ld(v[1], lanes + kColO + n + 16);
-                    tmem_wait_ld(v[0]);
-                    tmem_wait_ld(v[1]);
+                    uint32_t v[32];
+                    tmem_ld32(v, lanes + kColO + n);
+                    tmem_wait_ld(v);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 z = *reinterpret_cast<const float4 *>(sh.z0_v() + n + j);
-                        const uint32_t *o = &v[j / 16][j % 16];
-                        const float4 x = make_float4(fmaf(l, z.x, kPreUnit * __uint_as_float(o[0])), fmaf(l, z.y, kPreUnit * __uint_as_float(o[1])),
-                                                     fmaf(l, z.z, kPreUnit * __uint_as_float(o[2])), fmaf(l, z.w, kPreUnit * __uint_as_float(o[3])));
-                        *reinterpret_cast<float4 *>(row + 4 + n + j) = dead ? make_float4(0.f, 0.f, 0.f, 0.f) : x;
+                    for (int k = 0; k < 32; k += 16) {
+                        float4 z[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) z[j] = *reinterpret_cast<const float4 *>(sh.z0_v() + n + k + 4 * j);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t *o = &v[k + 4 * j];
+                            const float4 x = make_float4(fmaf(l, z[j].x, kPreUnit * __uint_as_float(o[0])), fmaf(l, z[j].y, kPreUnit * __uint_as_float(o[1])),
+                                                         fmaf(l, z[j].z, kPreUnit * __uint_as_float(o[2])), fmaf(l, z[j].w, kPreUnit * __uint_as_float(o[3])));
+                            *reinterpret_cast<float4 *>(row + 4 + n + k + 4 * j) = dead ? make_float4(0.f, 0.f, 0.f, 0.f) : x;
+                        }
                     }
                 }
                 fence_async_shared();
@@ -443,90 +448,74 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             }
         } else if (warp == 12) {
             // -------------------------------------------------------------------------- S = Q x^T
-            constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kPreTok / 2, true), lo_desc = pre_mma_desc(kPreRows, kPreTok / 2, true, true);
-            int i = 0;
-            int issued = min(2, n_tiles);
+            constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kPreTok, true), lo_desc = pre_mma_desc(kPreRows, kPreTok, true, true);
+            int i = 0, issued = min(kPreK, n_tiles);
             if (elect_one())
                 for (int k = 0; k < issued; ++k) load_tile(0, k);
             __syncwarp();
-            load_q(threadIdx.x - 256);
+            asm volatile("bar.sync 1, 160;" ::: "memory");   // Q is in place
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
-                const int tile = done + i, buf = tile & 1;
-                if (tile >= 2 && !(ok = mbar_wait(&sh.odone[buf], (tile >> 1 & 1) ^ 1, kStatVWait))) break;   // the weights in S's place are used
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    if (!(ok = mbar_wait(&sh.full[0][half], tile & 1, kStatKWait))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t d = tmem + kColS + kPreTok * buf + (kPreTok / 2) * half;
-                        const uint64_t qd = k_major_desc(&sh.q[0][0][0], kPreRows * 16, 128), xd = mn_major_desc(&sh.x[0][half][0][0][0], 128, kD * 16);
+                const int tile = done + i, slot = tile % kPreK, buf = tile % kPreV;
+                if (!(ok = mbar_wait_both(&sh.kfull[slot], tile / kPreK & 1, tile >= kPreV ? &sh.odone[buf] : nullptr, (tile / kPreV & 1) ^ 1, kStatKWait)))
+                    break;   // K is there, the weights in S's place are used
+                tc_fence_after();
+                if (elect_one()) {
+                    if (issued < n_tiles) load_tile(0, issued);   // the words of this tile are read
+                    const uint32_t d = tmem + kColS + kPreTok * buf;
+                    const uint64_t xd = mn_major_desc(&sh.k[slot][0][0][0], 128, kD * 16);
 #pragma unroll
-                        for (int n = 0; n < kD / 16; ++n) mma_smem(d, qd + 2 * kPreRows * n, xd + 16 * n, hi_desc, n > 0);
+                    for (int n = 0; n < kD / 16; ++n) mma_tmem(d, tmem + kColQ + 8 * n, xd + 16 * n, hi_desc, n > 0);
 #pragma unroll
-                        for (int n = 0; n < kD / 16; ++n) mma_smem(d, qd + 2 * kPreRows * n, xd + (kPreTok / 16) * kD + 16 * n, lo_desc, true);
-                        mma_commit(&sh.read[0][half]);
-                        if (half) mma_commit(&sh.sdone[buf]);
-                    }
-                    __syncwarp();
+                    for (int n = 0; n < kD / 16; ++n) mma_tmem(d, tmem + kColQ + 8 * n, xd + (kPreTok / 8) * kD + 16 * n, lo_desc, true);
+                    mma_commit(&sh.kread[slot]);
+                    mma_commit(&sh.sdone[buf]);
                 }
-                if (!ok) break;
-                if (issued < n_tiles) {   // the words of this tile are read
-                    if (elect_one()) load_tile(0, issued);
-                    ++issued;
-                }
+                ++issued;
                 __syncwarp();
             }
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             if (sh.dead) {   // products and copies in flight
-                for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k & 1], k >> 1 & 1, kStatDrain);
-                if (!ok) mbar_wait(&sh.read[0][0], done + i & 1, kStatDrain);   // the first half of the tile at which this warp gave up, if it was issued
-                for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k & 1], k >> 1 & 1, kStatDrain);
+                for (int k = done + max(i - kPreV, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k % kPreV], k / kPreV & 1, kStatDrain);
+                issued = min(issued, n_tiles);
+                for (int k = done + max(issued - kPreK, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k % kPreK], k / kPreK & 1, kStatDrain);
             }
         } else {
             // -------------------------------------------------------------------------- O += P y
             constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kD, false), lo_desc = pre_mma_desc(kPreRows, kD, false, true);
-            int i = 0;
-            int issued = min(2, n_tiles);
+            int i = 0, issued = min(kPreK, n_tiles);
             if (elect_one())
                 for (int k = 0; k < issued; ++k) load_tile(1, k);
             __syncwarp();
-            load_q(threadIdx.x - 256);
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
-                const int tile = done + i, buf = tile & 1;
-                if (!(ok = mbar_wait(&sh.pfull[buf], tile >> 1 & 1, kStatVWait))) break;
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    if (!(ok = mbar_wait(&sh.full[1][half], tile & 1, kStatVWait))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t pa = tmem + kColS + kPreTok * buf + (kPreTok / 4) * half;
-                        const uint64_t yd = k_major_desc(&sh.x[1][half][0][0][0], kD * 16, 128);
+                const int tile = done + i, buf = tile % kPreV;
+                if (!(ok = mbar_wait(&sh.vfull[buf], tile / kPreV & 1, kStatVWait))) break;
+                if (elect_one() && issued < n_tiles) load_tile(1, issued);
+                ++issued;
+                __syncwarp();
+                if (!(ok = mbar_wait(&sh.pfull[buf], tile / kPreV & 1, kStatVWait))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t pa = tmem + kColS + kPreTok * buf;
+                    const uint64_t yd = k_major_desc(&sh.v[buf][0][0][0], kD * 16, 128);
 #pragma unroll
-                        for (int n = 0; n < kPreTok / 32; ++n) {
-                            mma_tmem(tmem + kColO, pa + 8 * n, yd + 2 * kD * n, hi_desc, i > 0 || half > 0 || n > 0);
-                            mma_tmem(tmem + kColO, pa + 8 * n, yd + (kPreTok / 16) * kD + 2 * kD * n, lo_desc, true);
-                        }
-                        mma_commit(&sh.read[1][half]);
-                        if (half) mma_commit(&sh.odone[buf]);
+                    for (int n = 0; n < kPreTok / 16; ++n) {
+                        mma_tmem(tmem + kColO, pa + 8 * n, yd + 2 * kD * n, hi_desc, i > 0 || n > 0);
+                        mma_tmem(tmem + kColO, pa + 8 * n, yd + (kPreTok / 8) * kD + 2 * kD * n, lo_desc, true);
+                        mma_tmem(tmem + kColO, pa + kPreTok / 2 + 8 * n, yd + 2 * kD * n, lo_desc, true);
                     }
-                    __syncwarp();
-                }
-                if (!ok) break;
-                if (issued < n_tiles) {   // the words of this tile are read
-                    if (elect_one()) load_tile(1, issued);
-                    ++issued;
+                    mma_commit(&sh.odone[buf]);
                 }
                 __syncwarp();
             }
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             if (sh.dead) {
-                for (int k = done + max(i - 2, 0); k < done + i; ++k) mbar_wait(&sh.odone[k & 1], k >> 1 & 1, kStatDrain);
-                if (!ok) mbar_wait(&sh.read[1][0], done + i & 1, kStatDrain);
-                for (int k = done + max(issued - 2, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k & 1], k >> 1 & 1, kStatDrain);
+                for (int k = done + max(i - kPreV, 0); k < done + i; ++k) mbar_wait(&sh.odone[k % kPreV], k / kPreV & 1, kStatDrain);
+                issued = min(issued, n_tiles);
+                for (int k = done + max(issued - kPreK, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k % kPreK], k / kPreK & 1, kStatDrain);
             }
         }
         done += n_tiles;
