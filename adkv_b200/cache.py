@@ -202,6 +202,8 @@ class KVCacheLayer:
         ``(output [B, Hq, D], weights)``; ``weights`` is None for the fused step."""
         B, Hq, Tq, D = query_states.shape
         H, Tk = key_states.shape[1], key_states.shape[2]
+        if self._prefix is not None and attention_mask is not None:
+            raise ValueError("a layer behind a shared prefix takes no mask")
         if Tq != 1 or Tk != 1:
             raise ValueError(f"a decode step takes exactly one new token per sequence, not {Tq} queries / {Tk} keys")
         if Hq % H:
@@ -216,8 +218,6 @@ class KVCacheLayer:
         if mask is not None and mask.dim() == 4:
             mask = mask[:, :, 0, :]
         if self._prefix is not None:
-            if mask is not None:
-                raise ValueError("a layer behind a shared prefix takes no mask")
             need = gemv.prefix_scratch_bytes(B, Hq, self._prefix)
             if self._scratch is None or self._scratch.numel() < need:
                 self._scratch = torch.empty(need, dtype=torch.uint8, device=self._geom[3])

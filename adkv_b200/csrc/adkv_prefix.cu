@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         const int unit = int(at / plan.n_int), i0 = int(at % plan.n_int), i1 = int(min((long long)plan.n_int, i0 + last - at));
         at += i1 - i0;
         const int rt = unit % plan.row_tiles, h = unit / plan.row_tiles;
-        const int t0 = i0 * plan.interval, ntok = min(a.tokens, i1 * plan.interval) - t0, n_tiles = (ntok + kPreTok - 1) / kPreTok;
+        const int t0 = i0 * plan.interval, ntok = int(min((long long)a.tokens, (long long)i1 * plan.interval)) - t0, n_tiles = (ntok + kPreTok - 1) / kPreTok;
         const int rows = min(kPreRows, a.rows - rt * kPreRows);
         // packed tile i of K or V, by one lane of a warp
         const auto load_tile = [&](int tensor, int i) {

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
     }
     const auto finish = [&](const Place &p, int st) {
         int pos = a.start + p.t;
-        if (a.positions) pos = a.per_token ? a.positions[p.b * a.T + p.t] : a.positions[p.b] + p.t;
+        if (a.positions) pos = a.per_token ? a.positions[p.b * a.T + p.t] : int(uint32_t(a.positions[p.b]) + uint32_t(p.t));   // behind the largest int: negative
         float c[UNITS][4], s[UNITS][4];
         const bool inside = pos >= 0 && pos < a.table_rows;
         if (!inside && threadIdx.x == 0 && blockIdx.y == 0) atomicExch(&g_status, kStatPosition);

@@ -99,7 +99,7 @@ def process_logits(logits, *, history: torch.Tensor | None = None, history_lens:
     * plus ``bias`` (float32 ``[V]`` or ``[B, V]``);
     * -inf where bit ``v % 32`` of ``mask[b, v // 32]`` (int32, at least ``ceil(V / 32)`` words a row) is not set.
 
-    ``out``: of the logits' type and shape, may be ``logits`` itself.  ``tokens`` int32 ``[B]``: the lowest index of the largest element of
+    ``out``: of the logits' type and shape, may be ``logits`` itself but not overlap them in another way.  ``tokens`` int32 ``[B]``: the lowest index of the largest element of
     ``out`` (a NaN counts as the largest), -1 for a row of nothing but -inf."""
     native = out is None and _lib.host()
     if native:                                  # as in norm_rope_qkv
