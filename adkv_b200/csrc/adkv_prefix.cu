@@ -541,11 +541,56 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
 // =========================================================================================
 // The tokens that a sequence has cached itself, from the state behind the prefix, and the new one: one CTA per stream, as in the fused
 // step of adkv_fused.cu.  Its part comes behind those of the prefix's runs.
+// Where a row has few parts the kernel adds them up itself, with a part's 128 sums 16 bytes a lane: a launch less, 3 us on the host, which
+// bounds small calls, and on the device 14.0 -> 12.9 us for 3 parts, 57.9 -> 57.5 for 4 of eight heads, 48.1 us
+// either way for 8; with 18 parts 37.0 -> 42.3 us, with 37 36.3 -> 40.9, so those are left to the four warps a row of the join.
+constexpr int kFoldParts = 8, kFoldLoads = 4;   // kFoldLoads: parts that are under way at once
 template <int G, int TOK>
 struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
     float *part;   // [G][kPartStride]
-    __device__ __forceinline__ void store(const VArgs &, int, int, int c0, const float (&acc)[G][4]) const
+    int fold;      // parts of the prefix's runs, in front of this one, that are added up here; -1: the join does it
+    __device__ __forceinline__ void store(const VArgs &a, int b, int h, int c0, const float (&acc)[G][4]) const
     {
+        if (fold >= 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix kernel's results
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float m = this->m[g], l = this->denominator(g);
+                float4 o = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+                const float *base = part - size_t(fold) * G * kPartStride + g * kPartStride;
+#pragma unroll 1
+                for (int j0 = 0; j0 < fold; j0 += kFoldLoads) {
+                    float2 part_ml[kFoldLoads];
+                    float4 x[kFoldLoads];
+#pragma unroll
+                    for (int u = 0; u < kFoldLoads; ++u) {
+                        const float *p = base + min(j0 + u, fold - 1) * (G * kPartStride);
+                        part_ml[u] = *reinterpret_cast<const float2 *>(p);
+                        x[u] = *reinterpret_cast<const float4 *>(p + 4 + c0);
+                    }
+                    float top = m;
+#pragma unroll
+                    for (int u = 0; u < kFoldLoads; ++u) top = fmaxf(top, part_ml[u].x);
+                    const float corr = m == -INFINITY ? 0.f : exp2f(m - top);
+                    m = top;
+                    l *= corr;
+                    o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr;
+#pragma unroll
+                    for (int u = 0; u < kFoldLoads; ++u)
+                        if (j0 + u < fold) {
+                            const float w = part_ml[u].x == -INFINITY ? 0.f : exp2f(part_ml[u].x - top);
+                            l = fmaf(part_ml[u].y, w, l);   // a NaN: the part could not be finished
+                            o.x = fmaf(x[u].x, w, o.x);
+                            o.y = fmaf(x[u].y, w, o.y);
+                            o.z = fmaf(x[u].z, w, o.z);
+                            o.w = fmaf(x[u].w, w, o.w);
+                        }
+                }
+                __half *out = a.out + (size_t(b) * a.Hq + h * G + g) * kD + c0;
+                *reinterpret_cast<uint2 *>(out) = make_uint2(pack_half2(o.x / l, o.y / l), pack_half2(o.z / l, o.w / l));
+            }
+            return;
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float l = this->denominator(g);
@@ -554,10 +599,14 @@ struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
         }
     }
     // a bounded wait gave up, or the length did not fit: the result is NaN
-    __device__ __forceinline__ void give_up(int c0) const
+    __device__ __forceinline__ void give_up(const VArgs &a, int b, int h, int c0) const
     {
 #pragma unroll 1
         for (int g = 0; g < G; ++g) {
+            if (fold >= 0) {
+                *reinterpret_cast<uint2 *>(a.out + (size_t(b) * a.Hq + h * G + g) * kD + c0) = make_uint2(0x7fff7fffu, 0x7fff7fffu);
+                continue;
+            }
             if (c0 == 0) *reinterpret_cast<float2 *>(part + g * kPartStride) = make_float2(-INFINITY, __int_as_float(0x7fc00000));
             *reinterpret_cast<float4 *>(part + g * kPartStride + 4 + c0) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -572,9 +621,9 @@ __device__ __forceinline__ int prefix_parts(const PrefixPlan &plan, int b, int h
 }
 
 template <int BITS, int G, int TOK>
-__global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, const float *__restrict__ k_state, const float *__restrict__ v_state,
+__global__ void __launch_bounds__(64, G == 8 ? 6 : 10) prefix_own_kernel(KArgs ka, VArgs va, const float *__restrict__ k_state, const float *__restrict__ v_state,
                                                         const int *__restrict__ seq_lens, float scaling, float *__restrict__ scratch,
-                                                        const __grid_constant__ PrefixPlan plan)
+                                                        const __grid_constant__ PrefixPlan plan, int fold)
 {
     constexpr int ST = TOK == 64 ? 2 : 3;   // tiles in flight
     __shared__ alignas(128) uint8_t kbuf[ST * Tile<BITS, TOK>::BYTES];
@@ -613,10 +662,12 @@ __global__ void __launch_bounds__(64) prefix_own_kernel(KArgs ka, VArgs va, cons
         src.scale2 = scaling * 1.4426950408889634f;
         src.n_tiles = (ka.T + TOK - 1) / TOK;
         src.t_begin = 0;
-        src.part = scratch + (size_t(bh) * plan.n_parts + prefix_parts(plan, b, h, G)) * G * kPartStride;
+        const int n = prefix_parts(plan, b, h, G);
+        src.part = scratch + (size_t(bh) * plan.n_parts + n) * G * kPartStride;
+        src.fold = fold ? n : -1;
         src.init();
         if (fits) v_warp<BITS, G, kArithFma, Src, ST, false, BITS == 4 && G == 1, TOK>(va, seg, b, h, lane, vbuf, vbar, wts, src);
-        else src.give_up(4 * lane);
+        else src.give_up(va, b, h, 4 * lane);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");   // what waits for this kernel waits for the prefix kernel, too
 }
@@ -740,14 +791,14 @@ static int launch_beside(void (*kernel)(Params...), int grid, int block, cudaStr
 
 template <int BITS, int G>
 static int launch_own(const KArgs &ka, const VArgs &va, const float *k_state, const float *v_state, const int *seq_lens, float scaling,
-                      float *scratch, const PrefixPlan &plan, int B, int most, cudaStream_t s)
+                      float *scratch, const PrefixPlan &plan, int B, int most, int fold, cudaStream_t s)
 {
     // Tiles of 32 tokens where a sequence is short, and with eight query heads, 4-bit, where 64 leave room for fewer CTAs (see short_tiles in
     // adkv_fused.cu).  Whole step behind 64 tokens, 64 -> 32 tokens a tile: 64 x 32 heads, 100 tokens 32.2 -> 31.2 us, 600 81.9 -> 81.9 us; 32 x 8 of four
     // heads, 2-bit, 100 20.5 -> 19.9 us, 600 56.4 -> 60.9 us; 128 x 8 of eight heads 100 49.0 -> 42.4 us, 600 118.9 -> 114.2 us, 1500 243 -> 252 us.
     const auto kernel = most <= (BITS == 4 && G == 8 ? 1000 : 128) ? prefix_own_kernel<BITS, G, 32> : prefix_own_kernel<BITS, G, 64>;
-    if (plan.ctas) return launch_beside(kernel, B * ka.Hkv, 64, s, ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
-    kernel<<<B * ka.Hkv, 64, 0, s>>>(ka, va, k_state, v_state, seq_lens, scaling, scratch, plan);
+    if (plan.ctas) return launch_beside(kernel, B * ka.Hkv, 64, s, ka, va, k_state, v_state, seq_lens, scaling, scratch, plan, fold);
+    kernel<<<B * ka.Hkv, 64, 0, s>>>(ka, va, k_state, v_state, seq_lens, scaling, scratch, plan, fold);
     return launch_status();
 }
 
@@ -821,10 +872,11 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     if (plan.ctas)
         if (int rc = bits == 4 ? launch_prefix<4>(pa, plan, s) : launch_prefix<2>(pa, plan, s)) return rc;
     const int most = seq_lens ? int(std::min((long long)n_super_cap * (32 / bits), 1ll << 30)) : T;   // own tokens of a sequence, at most
+    const int fold = plan.n_parts - 1 <= kFoldParts;
     int rc = 0;
     ADKV_DISPATCH_H(bits, G, (rc = launch_own<BITS, G>(ka, va, static_cast<const float *>(prefix->k_tail), static_cast<const float *>(prefix->v_tail),
-                                                         static_cast<const int *>(seq_lens), scaling, pa.scratch, plan, B, most, s)))
-    if (rc) return rc;
+                                                         static_cast<const int *>(seq_lens), scaling, pa.scratch, plan, B, most, fold, s)))
+    if (rc || fold) return rc;
     return launch_beside(prefix_join_kernel, B * Hq, 32 * kJoinWarps, s, pa.scratch, static_cast<__half *>(out), Hq, Hkv, plan);
 }
 

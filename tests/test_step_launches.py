@@ -26,8 +26,12 @@ def test_three_launches_behind_one_another():
     assert rc == 0 and names(got) == ["prefix_kernel", "prefix_own", "prefix_join"]
     assert [g[3] for g in got] == [False, True, True]
     assert [g[1] for g in got[1:]] == [4 * 8, 4 * 8]
-    rc, got = prefix(4, 8, 8, 0, 0)                       # nothing in front: two
-    assert rc == 0 and names(got) == ["prefix_own", "prefix_join"] and [g[3] for g in got] == [False, True]
+    rc, got = prefix(4, 8, 8, 576, 64)                    # nine parts
+    assert rc == 0 and len(got) == 3
+    rc, got = prefix(4, 8, 8, 512, 64)                    # few parts of a row: no join
+    assert rc == 0 and names(got) == ["prefix_kernel", "prefix_own"] and [g[3] for g in got] == [False, True]
+    rc, got = prefix(4, 8, 8, 0, 0)                       # nothing in front
+    assert rc == 0 and names(got) == ["prefix_own"] and not got[0][3]
     assert prefix(0, 8, 8, 1000, 64) == (0, [])
 
 
