@@ -32,7 +32,7 @@
 namespace adkv {
 
 constexpr int kPreTok = 32, kPreRows = 128;   // tokens of a tile, query rows of a CTA
-constexpr int kPreK = 4, kPreV = 2;           // tiles of K and of V (of S, weights) that are on their way at once
+constexpr int kPreWords = 4, kPreKV = 3, kPreP = 2;   // tiles of words, of K and of V values, and of S and weights that are on their way at once
 constexpr int kPreWarps = 14;                 // 0-3: K, 4-7: V (a channel a thread), 8-11: softmax (a row a thread), 12, 13: products
 constexpr int kPreThreads = 32 * kPreWarps;
 constexpr float kPreUnit = 16.f;              // values are held in units of this
@@ -64,19 +64,19 @@ struct PrefixPlan {
 template <int BITS>
 struct PrefixShared {
     // values of a tile: [token / 8][channel][token % 8], the rounded ones in the first half and the remainders in the other
-    alignas(128) __half k[kPreK][2 * kPreTok / 8][kD][8];
-    alignas(128) __half v[kPreV][2 * kPreTok / 8][kD][8];
-    alignas(128) uint32_t words[2][kPreK][kPreTok * BITS / 32][kD];   // packed tiles of K and V
+    alignas(128) __half k[kPreKV][2 * kPreTok / 8][kD][8];
+    alignas(128) __half v[kPreKV][2 * kPreTok / 8][kD][8];
+    alignas(128) uint32_t words[2][kPreWords][kPreTok * BITS / 32][kD];   // packed tiles of K and V
     alignas(16) float base[kPreRows];                    // what the zero points of K before the run add to every logit of a row
     // The results of the run lie in k and v, a row every kPartStride floats (no two of eight in the same banks), and the zero points of V
     // before the run in the last row of words, where only their own thread has read.
     __device__ float *row(int r) { return reinterpret_cast<float *>(&k[0][0][0][0]) + r * kPartStride; }
-    __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][kPreK - 1][kPreTok * BITS / 32 - 1][0]); }
+    __device__ float *z0_v() { return reinterpret_cast<float *>(&words[1][kPreWords - 1][kPreTok * BITS / 32 - 1][0]); }
     uint32_t tmem;
     int dead;                                            // a bounded wait gave up
-    // of tile i, slot i % kPreK or i % kPreV: words are there; K values are there, have been read; V values are there; S is there; weights
-    // are there; O is added up (and V and the weights have been read)
-    uint64_t loaded[2][kPreK], kfull[kPreK], kread[kPreK], vfull[kPreV], sdone[kPreV], pfull[kPreV], odone[kPreV];
+    // of a tile: words are there; K values are there, have been read; V values are there; S is there; weights are there; O is added up (and
+    // V and the weights have been read)
+    uint64_t loaded[2][kPreWords], kfull[kPreKV], kread[kPreKV], vfull[kPreKV], sdone[kPreP], pfull[kPreP], odone[kPreKV];
 };
 
 // K-major shared-memory matrix without swizzle: element (m, k) lies at (m / 8) * m_stride + (k / 8) * k_stride + (m % 8) * 16 + (k % 8) * 2.
@@ -179,24 +179,26 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PrefixShared<BITS> &sh = *reinterpret_cast<PrefixShared<BITS> *>(smem_raw);
     constexpr int TPW = Codec<BITS>::TPW, WORDS = kPreTok / TPW;                // word rows of a tile
-    constexpr uint32_t kColQ = 0, kColS = kD / 2, kColO = kColS + kPreV * kPreTok, kColumns = 256;   // Q; S, with the weights in its place; O
+    constexpr uint32_t kColQ = 0, kColS = kD / 2, kColO = kColS + kPreP * kPreTok, kColumns = 256;   // Q; S, with the weights in its place; O
     static_assert(kColO + kD <= kColumns, "columns of tensor memory");
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hkv;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the sequences' own tokens may be scanned beside this kernel
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kPreK; ++i) {
+        for (int i = 0; i < kPreWords; ++i) {
             mbar_init(&sh.loaded[0][i], 1);
             mbar_init(&sh.loaded[1][i], 1);
+        }
+        for (int i = 0; i < kPreKV; ++i) {
             mbar_init(&sh.kfull[i], 4);
             mbar_init(&sh.kread[i], 1);
-        }
-        for (int i = 0; i < kPreV; ++i) {
             mbar_init(&sh.vfull[i], 4);
+            mbar_init(&sh.odone[i], 1);
+        }
+        for (int i = 0; i < kPreP; ++i) {
             mbar_init(&sh.sdone[i], 1);
             mbar_init(&sh.pfull[i], 4);
-            mbar_init(&sh.odone[i], 1);
         }
         sh.dead = 0;
         mbar_init_fence();
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         const int rows = min(kPreRows, a.rows - rt * kPreRows);
         // packed tile i of K or V, by one lane of a warp
         const auto load_tile = [&](int tensor, int i) {
-            const int slot = (done + i) % kPreK, n = min(WORDS, (ntok + TPW - 1) / TPW - i * WORDS);
+            const int slot = (done + i) % kPreWords, n = min(WORDS, (ntok + TPW - 1) / TPW - i * WORDS);
             uint64_t *bar = &sh.loaded[tensor][slot];
             mbar_expect_tx(bar, n * kD * 4);
             bulk_load(&sh.words[tensor][slot][0][0], a.cache[tensor] + (size_t(h) * a.n_super_cap + t0 / TPW + size_t(i) * WORDS) * kD * 4, n * kD * 4, bar);
@@ -255,11 +257,11 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             bool tame = true;   // no scale of the warp was outside its interval when last looked at
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i) {
-                const int tile = done + i, slot = tile % kPreK, buf = tile % kPreV;
+                const int tile = done + i, slot = tile % kPreWords, buf = tile % kPreKV;
                 // the words have come, and the products that read this buffer before are done
-                uint64_t *freed = which ? (tile >= kPreV ? &sh.odone[buf] : nullptr) : (tile >= kPreK ? &sh.kread[slot] : nullptr);
-                if (!(ok = mbar_wait_both(&sh.loaded[which][slot], tile / kPreK & 1, freed, (tile / (which ? kPreV : kPreK) & 1) ^ 1, kStatKWait))) break;
-                uint8_t *dst = reinterpret_cast<uint8_t *>(which ? &sh.v[buf][0][c][0] : &sh.k[slot][0][c][0]);
+                uint64_t *freed = tile < kPreKV ? nullptr : which ? &sh.odone[buf] : &sh.kread[buf];
+                if (!(ok = mbar_wait_both(&sh.loaded[which][slot], tile / kPreWords & 1, freed, (tile / kPreKV & 1) ^ 1, kStatKWait))) break;
+                uint8_t *dst = reinterpret_cast<uint8_t *>(which ? &sh.v[buf][0][c][0] : &sh.k[buf][0][c][0]);
                 const uint32_t *row = &sh.words[which][slot][0][c];
                 const int left = ntok - i * kPreTok;
                 uint32_t w[WORDS];
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                     tame = __all_sync(kFull, least >= lo && most <= hi);
                 }
                 fence_async_shared();
-                warp_arrive(which ? &sh.vfull[buf] : &sh.kfull[slot], lane);
+                warp_arrive(which ? &sh.vfull[buf] : &sh.kfull[buf], lane);
             }
             if (which == 1) sh.z0_v()[c] = start;
             if (!ok && lane == 0) sh.dead = 1;
@@ -352,8 +354,8 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             asm volatile("bar.sync 1, 160;" ::: "memory");   // with the warp that issues the products
 #pragma unroll 1
             for (int i = 0; i < n_tiles && busy; ++i) {
-                const int tile = done + i, buf = tile % kPreV;
-                if (!(ok = mbar_wait(&sh.sdone[buf], tile / kPreV & 1, kStatLFullWait))) break;
+                const int tile = done + i, buf = tile % kPreP;
+                if (!(ok = mbar_wait(&sh.sdone[buf], tile / kPreP & 1, kStatLFullWait))) break;
                 tc_fence_after();
                 const uint32_t cols = lanes + kColS + kPreTok * buf;
                 const int left = ntok - i * kPreTok;
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                     const float corr = grown ? exp2_fast(m - top) : 1.f;
                     if (i > 0) {
                         // all sums so far are in: O can be changed
-                        if (!(ok = mbar_wait(&sh.odone[(tile - 1) % kPreV], (tile - 1) / kPreV & 1, kStatVWait))) break;
+                        if (!(ok = mbar_wait(&sh.odone[(tile - 1) % kPreKV], (tile - 1) / kPreKV & 1, kStatVWait))) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int n = 0; n < kD; n += 16) {
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                 warp_arrive(&sh.pfull[buf], lane, 1 + idle);
             }
             const int end = done + n_tiles - 1;
-            if (ok && busy) ok = mbar_wait(&sh.odone[end % kPreV], end / kPreV & 1, kStatVWait);
+            if (ok && busy) ok = mbar_wait(&sh.odone[end % kPreKV], end / kPreKV & 1, kStatVWait);
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             const bool dead = sh.dead != 0;
@@ -449,15 +451,16 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
         } else if (warp == 12) {
             // -------------------------------------------------------------------------- S = Q x^T
             constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kPreTok, true), lo_desc = pre_mma_desc(kPreRows, kPreTok, true, true);
-            int i = 0, issued = min(kPreK, n_tiles);
+            int i = 0, issued = min(kPreWords, n_tiles);
             if (elect_one())
                 for (int k = 0; k < issued; ++k) load_tile(0, k);
             __syncwarp();
             asm volatile("bar.sync 1, 160;" ::: "memory");   // Q is in place
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
-                const int tile = done + i, slot = tile % kPreK, buf = tile % kPreV;
-                if (!(ok = mbar_wait_both(&sh.kfull[slot], tile / kPreK & 1, tile >= kPreV ? &sh.odone[buf] : nullptr, (tile / kPreV & 1) ^ 1, kStatKWait)))
+                const int tile = done + i, slot = tile % kPreKV, buf = tile % kPreP;
+                uint64_t *freed = tile >= kPreP ? &sh.odone[(tile - kPreP) % kPreKV] : nullptr;
+                if (!(ok = mbar_wait_both(&sh.kfull[slot], tile / kPreKV & 1, freed, max(tile - kPreP, 0) / kPreKV & 1, kStatKWait)))
                     break;   // K is there, the weights in S's place are used
                 tc_fence_after();
                 if (elect_one()) {
@@ -477,28 +480,28 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             if (sh.dead) {   // products and copies in flight
-                for (int k = done + max(i - kPreV, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k % kPreV], k / kPreV & 1, kStatDrain);
+                for (int k = done + max(i - kPreP, 0); k < done + i; ++k) mbar_wait(&sh.sdone[k % kPreP], k / kPreP & 1, kStatDrain);
                 issued = min(issued, n_tiles);
-                for (int k = done + max(issued - kPreK, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k % kPreK], k / kPreK & 1, kStatDrain);
+                for (int k = done + max(issued - kPreWords, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[0][k % kPreWords], k / kPreWords & 1, kStatDrain);
             }
         } else {
             // -------------------------------------------------------------------------- O += P y
             constexpr uint32_t hi_desc = pre_mma_desc(kPreRows, kD, false), lo_desc = pre_mma_desc(kPreRows, kD, false, true);
-            int i = 0, issued = min(kPreK, n_tiles);
+            int i = 0, issued = min(kPreWords, n_tiles);
             if (elect_one())
                 for (int k = 0; k < issued; ++k) load_tile(1, k);
             __syncwarp();
 #pragma unroll 1
             for (; i < n_tiles; ++i) {
-                const int tile = done + i, buf = tile % kPreV;
-                if (!(ok = mbar_wait(&sh.vfull[buf], tile / kPreV & 1, kStatVWait))) break;
+                const int tile = done + i, buf = tile % kPreKV, place = tile % kPreP;
+                if (!(ok = mbar_wait(&sh.vfull[buf], tile / kPreKV & 1, kStatVWait))) break;
                 if (elect_one() && issued < n_tiles) load_tile(1, issued);
                 ++issued;
                 __syncwarp();
-                if (!(ok = mbar_wait(&sh.pfull[buf], tile / kPreV & 1, kStatVWait))) break;
+                if (!(ok = mbar_wait(&sh.pfull[place], tile / kPreP & 1, kStatVWait))) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t pa = tmem + kColS + kPreTok * buf;
+                    const uint32_t pa = tmem + kColS + kPreTok * place;
                     const uint64_t yd = k_major_desc(&sh.v[buf][0][0][0], kD * 16, 128);
 #pragma unroll
                     for (int n = 0; n < kPreTok / 16; ++n) {
@@ -513,9 +516,9 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             if (!ok && lane == 0) sh.dead = 1;
             __syncthreads();
             if (sh.dead) {
-                for (int k = done + max(i - kPreV, 0); k < done + i; ++k) mbar_wait(&sh.odone[k % kPreV], k / kPreV & 1, kStatDrain);
+                for (int k = done + max(i - kPreKV, 0); k < done + i; ++k) mbar_wait(&sh.odone[k % kPreKV], k / kPreKV & 1, kStatDrain);
                 issued = min(issued, n_tiles);
-                for (int k = done + max(issued - kPreK, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k % kPreK], k / kPreK & 1, kStatDrain);
+                for (int k = done + max(issued - kPreWords, 0); k < done + issued; ++k) mbar_wait(&sh.loaded[1][k % kPreWords], k / kPreWords & 1, kStatDrain);
             }
         }
         done += n_tiles;
