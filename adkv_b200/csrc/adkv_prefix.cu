@@ -545,9 +545,9 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
 // The tokens that a sequence has cached itself, from the state behind the prefix, and the new one: one CTA per stream, as in the fused
 // step of adkv_fused.cu.  Its part comes behind those of the prefix's runs.
 // Where a row has few parts the kernel adds them up itself, with a part's 128 sums 16 bytes a lane: a launch less, 3 us on the host, which
-// bounds small calls, and on the device 14.0 -> 12.9 us for 3 parts, 57.9 -> 57.5 for 4 of eight heads, 48.1 us
-// either way for 8; with 18 parts 37.0 -> 42.3 us, with 37 36.3 -> 40.9, so those are left to the four warps a row of the join.
-constexpr int kFoldParts = 8, kFoldLoads = 4;   // kFoldLoads: parts that are under way at once
+// bounds small calls, and on the device 14.0 -> 12.9 us for 3 parts, 55.7 -> 51.4 for 4 of eight heads, 47.5 us either way for 8; 17.9 ->
+// 18.9 for 8 of four heads, 37.5 -> 40.7 us for 18 of two, so the more are left to the four warps a row of the join.
+constexpr int kFoldParts = 8, kFoldLoads = 8;   // kFoldLoads: rows of parts that are under way at once
 template <int G, int TOK>
 struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
     float *part;   // [G][kPartStride]
@@ -555,42 +555,45 @@ struct OwnSrc : SoftmaxSrc<G, 1, false, TOK> {
     __device__ __forceinline__ void store(const VArgs &a, int b, int h, int c0, const float (&acc)[G][4]) const
     {
         if (fold >= 0) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix kernel's results
+            float m[G], l[G];
+            float4 o[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                float m = this->m[g], l = this->denominator(g);
-                float4 o = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
-                const float *base = part - size_t(fold) * G * kPartStride + g * kPartStride;
+                m[g] = this->m[g];
+                l[g] = this->denominator(g);
+                o[g] = make_float4(acc[g][0], acc[g][1], acc[g][2], acc[g][3]);
+            }
+            const float *base = part - size_t(fold) * G * kPartStride;
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix kernel's results
 #pragma unroll 1
-                for (int j0 = 0; j0 < fold; j0 += kFoldLoads) {
-                    float2 part_ml[kFoldLoads];
-                    float4 x[kFoldLoads];
+            for (int j0 = 0; j0 < fold; j0 += kFoldLoads / G) {
+                float2 part_ml[kFoldLoads];   // of all heads at once: the rounds of loads are what takes time
+                float4 x[kFoldLoads];
 #pragma unroll
-                    for (int u = 0; u < kFoldLoads; ++u) {
-                        const float *p = base + min(j0 + u, fold - 1) * (G * kPartStride);
-                        part_ml[u] = *reinterpret_cast<const float2 *>(p);
-                        x[u] = *reinterpret_cast<const float4 *>(p + 4 + c0);
-                    }
-                    float top = m;
-#pragma unroll
-                    for (int u = 0; u < kFoldLoads; ++u) top = fmaxf(top, part_ml[u].x);
-                    const float corr = m == -INFINITY ? 0.f : exp2f(m - top);
-                    m = top;
-                    l *= corr;
-                    o.x *= corr; o.y *= corr; o.z *= corr; o.w *= corr;
-#pragma unroll
-                    for (int u = 0; u < kFoldLoads; ++u)
-                        if (j0 + u < fold) {
-                            const float w = part_ml[u].x == -INFINITY ? 0.f : exp2f(part_ml[u].x - top);
-                            l = fmaf(part_ml[u].y, w, l);   // a NaN: the part could not be finished
-                            o.x = fmaf(x[u].x, w, o.x);
-                            o.y = fmaf(x[u].y, w, o.y);
-                            o.z = fmaf(x[u].z, w, o.z);
-                            o.w = fmaf(x[u].w, w, o.w);
-                        }
+                for (int u = 0; u < kFoldLoads; ++u) {
+                    const float *p = base + (min(j0 + u / G, fold - 1) * G + u % G) * kPartStride;
+                    part_ml[u] = *reinterpret_cast<const float2 *>(p);
+                    x[u] = *reinterpret_cast<const float4 *>(p + 4 + c0);
                 }
+#pragma unroll
+                for (int u = 0; u < kFoldLoads; ++u) {
+                    const int g = u % G;
+                    if (j0 + u / G < fold) {
+                        const float top = fmaxf(m[g], part_ml[u].x), corr = m[g] == -INFINITY ? 0.f : exp2f(m[g] - top),
+                                    w = part_ml[u].x == -INFINITY ? 0.f : exp2f(part_ml[u].x - top);
+                        m[g] = top;
+                        l[g] = fmaf(part_ml[u].y, w, l[g] * corr);   // a NaN: the part could not be finished
+                        o[g].x = fmaf(x[u].x, w, o[g].x * corr);
+                        o[g].y = fmaf(x[u].y, w, o[g].y * corr);
+                        o[g].z = fmaf(x[u].z, w, o[g].z * corr);
+                        o[g].w = fmaf(x[u].w, w, o[g].w * corr);
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
                 __half *out = a.out + (size_t(b) * a.Hq + h * G + g) * kD + c0;
-                *reinterpret_cast<uint2 *>(out) = make_uint2(pack_half2(o.x / l, o.y / l), pack_half2(o.z / l, o.w / l));
+                *reinterpret_cast<uint2 *>(out) = make_uint2(pack_half2(o[g].x / l[g], o[g].y / l[g]), pack_half2(o[g].z / l[g], o[g].w / l[g]));
             }
             return;
         }
