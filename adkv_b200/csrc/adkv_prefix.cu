@@ -675,7 +675,8 @@ __global__ void __launch_bounds__(64, G == 8 ? 6 : 10) prefix_own_kernel(KArgs k
         if (fits) v_warp<BITS, G, kArithFma, Src, ST, false, BITS == 4 && G == 1, TOK>(va, seg, b, h, lane, vbuf, vbar, wts, src);
         else src.give_up(va, b, h, 4 * lane);
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // what waits for this kernel waits for the prefix kernel, too
+    // What waits for this kernel waits for the prefix kernel, too.  One CTA sees to that: the others make room.
+    if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // out[b, hq] = sum_j x_j 2^(m_j - M) / sum_j l_j 2^(m_j - M) over the parts of a row.  Four warps share a row's parts, a part's 128 sums are
