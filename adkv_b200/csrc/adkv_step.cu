@@ -401,6 +401,92 @@ __global__ void __launch_bounds__(kLogitThreads, 2) process_logits_kernel(const 
     uint32_t top_key = 0;
     int top_at = a.V;
     uint4 top_pack = make_uint4(0, 0, 0, 0);
+    // Pack p of the row, the at-th of those that are counted; raw: what it holds, if all of it lies in the row.
+    const auto work = [&](auto whole_pack, int p, int at, const uint4 &raw) {
+        const int v = p * N - skew;                    // index of the pack's first element
+        constexpr bool all = decltype(whole_pack)::value;
+        float y[N];
+        if constexpr (all) {
+            Io::unpack(raw, y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = v + i >= 0 && v + i < a.V ? Io::load(x + v + i) : 0.f;
+        }
+        if (n_history) {
+            uint32_t w[N / PER], any = 0;
+#pragma unroll
+            for (int i = 0; i < N / PER; ++i) w[i] = 0;
+            if constexpr (N / PER >= 4) {
+#pragma unroll
+                for (int i = 0; i < N / PER; i += 4) {
+                    const uint4 c = *reinterpret_cast<const uint4 *>(counts + at * (N / PER) + i);
+                    w[i] = c.x; w[i + 1] = c.y; w[i + 2] = c.z; w[i + 3] = c.w;
+                }
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2 *>(counts + at * (N / PER));
+                w[0] = c.x; w[1] = c.y;
+            }
+#pragma unroll
+            for (int i = 0; i < N / PER; ++i) any |= w[i];
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t n = PER == 1 ? w[i / PER] : w[i / PER] >> (i % PER * 16) & 0xffffu;
+                    if (n) {
+                        const float z = y[i] > 0.f ? __fdiv_rn(y[i], rep) : __fmul_rn(y[i], rep);
+                        y[i] = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(n)), pres));
+                    }
+                }
+            }
+        }
+        if (bias) {
+            if (all && bias4) {
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                    const float4 z = *reinterpret_cast<const float4 *>(bias + v + i);
+                    y[i] = __fadd_rn(y[i], z.x); y[i + 1] = __fadd_rn(y[i + 1], z.y);
+                    y[i + 2] = __fadd_rn(y[i + 2], z.z); y[i + 3] = __fadd_rn(y[i + 3], z.w);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (all || (v + i >= 0 && v + i < a.V)) y[i] = __fadd_rn(y[i], bias[v + i]);
+            }
+        }
+        if (mask) {
+            const int first = max(v, 0);
+            const uint32_t w0 = mask[first >> 5], w1 = mask[min((first >> 5) + 1, n_words - 1)];
+            const uint32_t bits = __funnelshift_r(w0, w1, first & 31) << (first - v);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (!(bits >> i & 1)) y[i] = -INFINITY;
+        }
+        const uint4 packed = Io::pack(y);
+        if (all && same) {
+            *reinterpret_cast<uint4 *>(out + v) = packed;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (v + i >= 0 && v + i < a.V) Io::store(out + v + i, y[i]);
+        }
+        if (a.tokens) {   // the pack with the largest element so far, the first of them
+            Io::unpack(packed, y);   // as they have been rounded
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (v + i < 0 || v + i >= a.V) y[i] = -INFINITY;
+            }
+            float most = y[0];
+#pragma unroll
+            for (int i = 1; i < N; ++i) most = max_or_nan(most, y[i]);
+            const uint32_t key = key_of(most);
+            if (key > top_key || (key == top_key && v < top_at)) {
+                top_key = key;
+                top_at = v;
+                top_pack = packed;
+            }
+        }
+    };
     constexpr int kPacks = kLogitBytes / int(sizeof(Count)) / N;
     for (int p0 = 0; p0 < a.part; p0 += kPacks) {
         const int p1 = min(a.part, p0 + kPacks);
@@ -434,90 +520,15 @@ __global__ void __launch_bounds__(kLogitThreads, 2) process_logits_kernel(const 
             for (int u = 0; u < kLogitAhead; ++u) {
                 const int l = base + u * kLogitThreads, p = pack_of(l);
                 if (l >= p1 || p >= packs) break;
-                const int v = p * N - skew;                    // index of the pack's first element
-                const bool all = whole(p);
-                float y[N];
-                if (all) {
-                    Io::unpack(ahead[u], y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) y[i] = v + i >= 0 && v + i < a.V ? Io::load(x + v + i) : 0.f;
-                }
-                if (n_history) {
-                    uint32_t w[N / PER], any = 0;
-#pragma unroll
-                    for (int i = 0; i < N / PER; ++i) w[i] = 0;
-                    if constexpr (N / PER >= 4) {
-#pragma unroll
-                        for (int i = 0; i < N / PER; i += 4) {
-                            const uint4 c = *reinterpret_cast<const uint4 *>(counts + (l - p0) * (N / PER) + i);
-                            w[i] = c.x; w[i + 1] = c.y; w[i + 2] = c.z; w[i + 3] = c.w;
-                        }
-                    } else {
-                        const uint2 c = *reinterpret_cast<const uint2 *>(counts + (l - p0) * (N / PER));
-                        w[0] = c.x; w[1] = c.y;
-                    }
-#pragma unroll
-                    for (int i = 0; i < N / PER; ++i) any |= w[i];
-                    if (any) {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const uint32_t n = PER == 1 ? w[i / PER] : w[i / PER] >> (i % PER * 16) & 0xffffu;
-                            if (n) {
-                                const float z = y[i] > 0.f ? __fdiv_rn(y[i], rep) : __fmul_rn(y[i], rep);
-                                y[i] = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(n)), pres));
-                            }
-                        }
-                    }
-                }
-                if (bias) {
-                    if (all && bias4) {
-#pragma unroll
-                        for (int i = 0; i < N; i += 4) {
-                            const float4 z = *reinterpret_cast<const float4 *>(bias + v + i);
-                            y[i] = __fadd_rn(y[i], z.x); y[i + 1] = __fadd_rn(y[i + 1], z.y);
-                            y[i + 2] = __fadd_rn(y[i + 2], z.z); y[i + 3] = __fadd_rn(y[i + 3], z.w);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < N; ++i)
-                            if (all || (v + i >= 0 && v + i < a.V)) y[i] = __fadd_rn(y[i], bias[v + i]);
-                    }
-                }
-                if (mask) {
-                    const int at = max(v, 0);
-                    const uint32_t w0 = mask[at >> 5], w1 = mask[min((at >> 5) + 1, n_words - 1)];
-                    const uint32_t bits = __funnelshift_r(w0, w1, at & 31) << (at - v);
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (!(bits >> i & 1)) y[i] = -INFINITY;
-                }
-                const uint4 packed = Io::pack(y);
-                if (all && same) {
-                    *reinterpret_cast<uint4 *>(out + v) = packed;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (v + i >= 0 && v + i < a.V) Io::store(out + v + i, y[i]);
-                }
-                if (a.tokens) {   // the pack with the largest element so far, the first of them (a thread's packs come in order)
-                    Io::unpack(packed, y);   // as they have been rounded
-                    if (!all) {
-#pragma unroll
-                        for (int i = 0; i < N; ++i)
-                            if (v + i < 0 || v + i >= a.V) y[i] = -INFINITY;
-                    }
-                    float most = y[0];
-#pragma unroll
-                    for (int i = 1; i < N; ++i) most = max_or_nan(most, y[i]);
-                    const uint32_t key = key_of(most);
-                    if (key > top_key) {
-                        top_key = key;
-                        top_at = v;
-                        top_pack = packed;
-                    }
-                }
+                if (whole(p)) work(std::true_type{}, p, l - p0, ahead[u]);
             }
+        }
+        // the first and the last pack of the row, where some of their elements lie outside
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            const int p = k ? packs - 1 : 0, group = p >> 5, l = group >> log_ranks << 5 | (p & 31);
+            if (whole(p) || (k && packs == 1) || (group & int(ranks - 1)) != int(rank) || l < p0 || l >= p1) continue;
+            if (int(threadIdx.x) == (l - p0) % kLogitThreads) work(std::false_type{}, p, l - p0, make_uint4(0, 0, 0, 0));
         }
         __syncthreads();   // the counts are read
     }
