@@ -813,7 +813,7 @@ extern "C" {
 
 long long adkv_decode_attn_prefix_scratch_bytes(int B, int Hq, int Hkv, int prefix_tokens, int interval)
 {
-    if (B < 0 || Hq <= 0 || Hkv <= 0 || prefix_tokens < 0 || interval < 0 || Hq % Hkv != 0) return ADKV_E_SHAPE;
+    if (B < 0 || Hq <= 0 || Hkv <= 0 || prefix_tokens < 0 || interval < 0 || Hq % Hkv != 0 || (long long)B * Hq > 0x7fffffffll) return ADKV_E_SHAPE;
     const PrefixPlan plan = prefix_plan(prefix_tokens, interval, B, Hq / Hkv, Hkv);
     return (long long)B * Hq * plan.n_parts * kPartStride * (long long)sizeof(float);
 }
@@ -845,7 +845,7 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
         !aligned16(prefix->v_ckpt) || (reinterpret_cast<uintptr_t>(seq_lens) & 3u))
         return ADKV_E_ALIGN;
     const long long rows = (long long)B * G;
-    if (rows > (1 << 24)) return ADKV_E_SHAPE;
+    if (rows > (1 << 24) || (long long)B * Hq > 0x7fffffffll) return ADKV_E_SHAPE;
     const long long need = adkv_decode_attn_prefix_scratch_bytes(B, Hq, Hkv, P, iv);
     if (need > 0 && !scratch) return ADKV_E_NULL;
     if (scratch_bytes < need) return ADKV_E_SCRATCH;

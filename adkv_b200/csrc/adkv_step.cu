@@ -673,7 +673,7 @@ int adkv_process_logits(const void *x, long long stride_x, void *out, long long 
                         long long stride_bias, const void *mask, long long stride_mask, int B, int V, void *stream)
 {
     if (!x || !out) return ADKV_E_NULL;
-    if (B < 0 || V <= 0 || V > 0x7fff0000 || history_cap < 0 || B > 65535) return ADKV_E_SHAPE;
+    if (B < 0 || V <= 0 || V > 0x7fff0000 || history_cap < 0 || B > 65535 || (B > 1 && stride_out < V)) return ADKV_E_SHAPE;   // rows of out must lie apart
     if (type < ADKV_T_F16 || type > ADKV_T_F32) return ADKV_E_TYPE;
     const unsigned size = type == ADKV_T_F32 ? 4 : 2;
     if (!aligned_to(x, size) || !aligned_to(out, size) || !aligned_to(tokens, 4) || !aligned_to(history, 4) || !aligned_to(history_lens, 4) ||

@@ -342,7 +342,8 @@ int adkv_norm_rope_qkv(const void *qkv, long long stride_b, long long stride_t, 
  *   repetition, presence, frequency: float [B], or NULL: the number that follows.
  *   out  of the logits' type, may be the logits; tokens int32 [B] or NULL: the lowest index of the largest element of out (a NaN counts
  *         as the largest), -1 where every element is -inf.
- * fp32 arithmetic, rounded once at the end; rows need no alignment beyond their type's; B at most 65535. */
+ * fp32 arithmetic, rounded once at the end; rows need no alignment beyond their type's, those of out lie apart; B at
+ * most 65535. */
 int adkv_process_logits(const void *x, long long stride_x, void *out, long long stride_out, int type, void *tokens, const void *history,
                         long long stride_history, int history_cap, const void *history_lens, const void *repetition, float repetition1,
                         const void *presence, float presence1, const void *frequency, float frequency1, const void *bias,

@@ -121,6 +121,28 @@ def test_one_prefix_for_calls_of_different_sizes_and_its_owner_going_on():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 2])
+def test_first_own_token_by_append_and_by_prefill(bits):
+    """A token appended at index 0, quantised as a chunk of one, and appended by the step: the same codes and tails."""
+    c = Shared(bits, 4, 2, 100, 64, [0, 0, 0], seed=6)
+    tails, caches = [], []
+    for how in range(3):
+        kt, vt = c.prefix.start_tails(3)
+        kc, vc = torch.zeros_like(c.kc), torch.zeros_like(c.vc)
+        if how == 0:
+            gemv.append_kv_pair(kc, c.new[0], c.kp, kt, vc, c.new[1], c.vp, vt, 0, *c.bounds, bits=bits)
+        elif how == 1:
+            gemv.encode_kv_pair(kc, c.new[0], c.kp, vc, c.new[1], c.vp, *c.bounds, bits=bits, k_tail=kt, v_tail=vt, from_tail=True)
+        else:
+            gemv.decode_attn_prefix(c.q, c.prefix, kc, vc, *c.new, c.kp, c.vp, 0, SCALING, *c.bounds, k_tail=kt, v_tail=vt)
+        tails.append((kt, vt))
+        caches.append((kc, vc))
+    for other in (1, 2):
+        for a, b in zip(tails[0] + caches[0], tails[other] + caches[other]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_counts_of_32_bits():
     for V, L in ((70, 70000), (40000, 100000)):
         x, kw = logits_inputs(2, V, L, torch.float32)

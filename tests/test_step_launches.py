@@ -60,6 +60,14 @@ def test_ctas_of_the_prefix(B, Hq, Hkv, P, interval, ctas):
     assert rc == 0 and got[0][1] == ctas
 
 
+def test_more_than_a_launch_can_hold_is_refused():
+    assert prefix(1 << 24, 1, 1, 100, 32)[0] == 0 and prefix((1 << 24) + 1, 1, 1, 100, 32) == (-4, [])
+    assert prefix(1 << 20, 1 << 12, 1 << 12, 100, 32) == (-4, [])
+    assert run("adkv_decode_attn_prefix_scratch_bytes", 1 << 20, 1 << 12, 1 << 12, 100, 32)[0] == -4
+    assert run("adkv_process_logits", PTR, 8, PTR, 7, 0, PTR, None, 0, 0, None, None, 1.0, None, 0.0, None, 0.0, None, 0, None, 0, 2, 8, None) == (-4, [])
+    assert run("adkv_process_logits", PTR, 8, PTR, 7, 0, PTR, None, 0, 0, None, None, 1.0, None, 0.0, None, 0.0, None, 0, None, 0, 1, 8, None)[0] == 0
+
+
 def test_tiles_of_own_tokens():
     """Short sequences take tiles of 32 tokens, by what the cache has room for or the length given."""
     def tok(**kw):
