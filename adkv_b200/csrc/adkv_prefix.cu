@@ -46,6 +46,7 @@ struct PrefixArgs {
     float *scratch;                  // [B * Hkv, n_parts, G, kPartStride]
     int Hq, Hkv, rows, n_super_cap, n_ckpt_cap, tokens;
     float scaling, smin, smax;
+    bool mute_k;                     // self-test (ADKV_FLAG_SELFTEST_MUTE_K): the K warps do nothing, so the waits behind them run out
 };
 
 // How the prefix is laid over CTAs.  The intervals of all units (128 rows of one head) form one line, of which every CTA takes an equal
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
             PrefixChan ch{0.f, s * (1.f / kPreUnit), alpha, beta, fmaf(-beta, target, 1.0f)};
             bool tame = true;   // no scale of the warp was outside its interval when last looked at
 #pragma unroll 1
-            for (int i = 0; i < n_tiles; ++i) {
+            for (int i = which == 0 && a.mute_k ? n_tiles : 0; i < n_tiles; ++i) {
                 const int tile = done + i, slot = tile % kPreWords, buf = tile % kPreKV;
                 // the words have come, and the products that read this buffer before are done
                 uint64_t *freed = tile < kPreKV ? nullptr : which ? &sh.odone[buf] : &sh.kread[buf];
@@ -831,7 +832,7 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     if (int rc = check_common(B, Hq, Hkv, T, D, n_super_cap, bits, T + 1)) return rc;
     const int G = Hq / Hkv;
     if (G != 1 && G != 2 && G != 4 && G != 8) return ADKV_E_SHAPE;
-    if (flags & ~unsigned(ADKV_FLAG_TAIL_KEEP | ADKV_FLAG_FAST_REPLAY)) return ADKV_E_FLAGS;
+    if (flags & ~unsigned(ADKV_FLAG_TAIL_KEEP | ADKV_FLAG_FAST_REPLAY | ADKV_FLAG_SELFTEST_MUTE_K)) return ADKV_E_FLAGS;
     const int P = prefix->tokens, iv = prefix->interval;
     if (P < 0 || prefix->n_super_cap < 0 || iv < 0 || iv % kTileTok || prefix->n_ckpt_cap < 0) return ADKV_E_SHAPE;
     if (((long long)P + 32 / bits - 1) / (32 / bits) > prefix->n_super_cap) return ADKV_E_CAPACITY;
@@ -869,6 +870,7 @@ int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_ca
     pa.scaling = scaling;
     pa.smin = scale_min;
     pa.smax = scale_max;
+    pa.mute_k = flags & ADKV_FLAG_SELFTEST_MUTE_K;
     const bool keep = flags & ADKV_FLAG_TAIL_KEEP;
     const KArgs ka{pa.q, static_cast<uint8_t *>(k_cache), static_cast<const __half *>(k_new), pa.p[0], Hq, Hkv, T, n_super_cap, scale_min, scale_max, D,
                    static_cast<float *>(k_tail), keep};

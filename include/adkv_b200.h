@@ -103,7 +103,8 @@ extern "C" {
  * once, so whatever waits for logits waits for ever.  Each wait gives up after its 1 s limit (the tensor cores' kernel counts it
  * in cycles, 2e9), the kernels end normally, adkv_device_status reports a wait that ran out (3, or 1 to 4 of that kernel), nothing
  * is appended, and every element of `out` is NaN -- a segment that could not be finished marks its partial result instead of
- * leaving whatever the scratch memory held. */
+ * leaving whatever the scratch memory held.  Of adkv_decode_attn_prefix the K warps of the prefix: the same, but the sequences' own
+ * tokens are replayed and the new ones appended as always. */
 #define ADKV_FLAG_SELFTEST_MUTE_K 0x80000000u
 
 /* The five per-(kv head, channel) parameter tensors, fp16 [Hkv, D] each
@@ -309,7 +310,8 @@ long long adkv_decode_attn_prefix_scratch_bytes(int B, int Hq, int Hkv, int pref
  *   seq_lens          int32 [B] on the device: own tokens of each sequence, 0 or more; or NULL: T of each.  A length that does not fit
  *          the cache is reported by adkv_device_status (6): nothing is appended, the outputs of that sequence are NaN.
  *   scratch           at least adkv_decode_attn_prefix_scratch_bytes, 16-byte aligned, contents irrelevant; not for two calls at once.
- * Head dim 128, Hq / Hkv of 1, 2, 4 or 8; flags: ADKV_FLAG_TAIL_KEEP (ADKV_FLAG_FAST_REPLAY is implied). */
+ * Head dim 128, Hq / Hkv of 1, 2, 4 or 8; flags: ADKV_FLAG_TAIL_KEEP, and the self-test's
+ * (ADKV_FLAG_FAST_REPLAY is implied). */
 int adkv_decode_attn_prefix(const void *q, const adkv_prefix *prefix, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
                             const adkv_params *kp, const adkv_params *vp, void *k_tail, void *v_tail, const void *seq_lens, int T,
                             void *out, void *scratch, long long scratch_bytes, int B, int Hq, int Hkv, int D, int n_super_cap, int bits,

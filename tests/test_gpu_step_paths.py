@@ -1,6 +1,8 @@
 """Steps behind a shared prefix, rotation and logits where their host and device code can take another way: without the native host path, on
 another stream, with pieces of the prefix that cross from one head to the next, long own tokens, counts of 32 bits, offsets behind 2^31."""
+import ctypes
 import math
+import time
 
 import pytest
 import torch
@@ -118,6 +120,39 @@ def test_one_prefix_for_calls_of_different_sizes_and_its_owner_going_on():
         got, want = child.decode(*args, scaling=SCALING)[0], whole.decode(*args, scaling=SCALING)[0]
         assert ((got - want).abs() <= 2e-3 + 2e-3 * want.abs()).all()
         assert all(torch.equal(a, b) for a, b in zip(child.tails, whole.tails))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,P,interval,B", [(4, 300, 0, 2), (2, 300, 32, 130), (4, 3000, 64, 2)])
+def test_waits_that_run_out_end_the_step(bits, P, interval, B):
+    """The scans of the prefix's keys do nothing: every wait behind them ends after its second, the results are NaN, the own tokens and
+    the new one are cached as always, and the next step is as if nothing had been."""
+    c = Shared(bits, 4, 2, P, interval, [3] * B, seed=8)
+    before = _state(c)
+    good = c.step()
+    after = _state(c)
+    for t, b in zip((c.kc, c.vc, c.kt, c.vt), before):
+        t.copy_(b)
+    out = torch.zeros_like(good)
+    scratch = torch.zeros(gemv.prefix_scratch_bytes(B, 4, c.prefix), dtype=torch.uint8, device="cuda")
+    kp, vp = (_lib.Params(*[t.data_ptr() for t in p]) for p in (c.kp, c.vp))
+    assert gemv.device_status() == 0
+    t0 = time.perf_counter()
+    rc = _lib.load().adkv_decode_attn_prefix(
+        c.q.data_ptr(), ctypes.addressof(c.prefix.desc), c.kc.data_ptr(), c.vc.data_ptr(), c.new[0].data_ptr(), c.new[1].data_ptr(), ctypes.addressof(kp),
+        ctypes.addressof(vp), c.kt.data_ptr(), c.vt.data_ptr(), c.lens_gpu.data_ptr(), 0, out.data_ptr(), scratch.data_ptr(), scratch.numel(), B, 4, 2, D,
+        c.cap, bits, SCALING, *c.bounds, _lib.FLAG_SELFTEST_MUTE_K, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    torch.cuda.synchronize()
+    seconds = time.perf_counter() - t0
+    assert 1 <= gemv.device_status() <= 4 and gemv.device_status() == 0
+    assert torch.isnan(out).all()
+    assert 0.9 < seconds < 4.0, seconds
+    for t, b in zip(_state(c), after):
+        assert torch.equal(t, b)
+    for t, b in zip((c.kc, c.vc, c.kt, c.vt), before):
+        t.copy_(b)
+    assert torch.equal(c.step(scratch=scratch), good)
 
 
 @pytest.mark.gpu
