@@ -7,6 +7,7 @@
 // attribute look-ups and 30-argument ctypes call of the Python path took 24 us.
 //
 // The same for gemv.decode_attn_prefix, step.norm_rope_qkv and step.process_logits, whose Python paths take 42, 25 and 17 us.
+#include <ATen/EmptyTensor.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -62,6 +63,12 @@ struct Device {
         return true;
     }
 };
+
+// A tensor on the current device, as at::empty makes it but without its way through the dispatcher (0.5 us).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type)
+{
+    return at::detail::empty_generic(sizes, c10::GetAllocator(at::kCUDA), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
 
 // A tuple of tensors, or None.
 PyObject *results(std::initializer_list<at::Tensor> tensors)
@@ -218,7 +225,7 @@ PyObject *decode_prefix(PyObject *, PyObject *const *a, Py_ssize_t n)
         void *scratch;
         long long room = need;
         if (a[16] == Py_None) {
-            own = at::empty({need}, kc->options());
+            own = fresh({need}, at::kByte);
             scratch = own.data_ptr();
         } else {
             const at::Tensor *t = plain(a[16]);
@@ -312,8 +319,7 @@ PyObject *norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
                 if (!t || t->dim() != 1 || t->size(0) != D || reinterpret_cast<uintptr_t>(t->data_ptr()) % step) Py_RETURN_NONE;
                 weight[i] = t->data_ptr();
             }
-        const auto options = x->options().dtype(to);
-        const at::Tensor q = at::empty({B, Hq, T, D}, options), k = at::empty({B, Hkv, T, D}, options), v = at::empty({B, Hkv, T, D}, options);
+        const at::Tensor q = fresh({B, Hq, T, D}, to), k = fresh({B, Hkv, T, D}, to), v = fresh({B, Hkv, T, D}, to);
         void *const stream = c10::cuda::getCurrentCUDAStream(dev.index).stream();
         int rc;
         const void *const xp = x->data_ptr(), *const cp = cos->data_ptr(), *const sp = sin->data_ptr();
@@ -377,7 +383,7 @@ PyObject *logits(PyObject *, PyObject *const *a, Py_ssize_t n)
             if (!bias) Py_RETURN_NONE;
         }
         if (a[7] != Py_None && !(mask = rows(a[7], at::kInt, (V + 31) / 32))) Py_RETURN_NONE;
-        const at::Tensor out = at::empty({B, V}, x->options()), tokens = at::empty({B}, x->options().dtype(at::kInt));
+        const at::Tensor out = fresh({B, V}, x->scalar_type()), tokens = fresh({B}, at::kInt);
         void *const stream = c10::cuda::getCurrentCUDAStream(dev.index).stream();
         const void *const xp = x->data_ptr(), *const hp = history ? history->data_ptr() : nullptr, *const mp = mask ? mask->data_ptr() : nullptr;
         int rc;

@@ -578,7 +578,7 @@ static int launch_rope_kernel(const RopeArgs &a, dim3 grid, cudaStream_t s)
 {
     constexpr int bytes = rope_stages<D, In>() * rope_slot_bytes<D, In>();
     const auto kernel = norm_rope_kernel<D, In, Out>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return launch_status();
+    if (bytes > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return launch_status();
     kernel<<<grid, kRopeThreads, bytes, s>>>(a);
     return launch_status();
 }
