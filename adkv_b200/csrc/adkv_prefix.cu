@@ -742,6 +742,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const floa
 
 // Two CTAs share an SM, 296 places.  A run costs, besides its tokens, what filling and emptying the pipeline and storing the result take, about
 // as long as 300 tokens: so either every unit gets the same number of CTAs, or the line is cut evenly and most CTAs come to have two runs.
+// CTAs of own tokens find room on an SM once it has only one of the prefix's.  So a unit gets no more CTAs than its longest run asks for (64
+// intervals: eight of eight, not nine of seven or eight): 64 x 32 heads behind 8192 tokens, 128 of their own 86.4 -> 82.8 us, 16 behind 2047,
+// 200 47.8 -> 37.0, 32 x 16 of two heads behind 8192, 10 52.7 -> 47.1; without own tokens 128 x 32 heads 74.9 -> 78.6.  Up to 256 streams, which the
+// free places can take in, 32 are left free always: 32 x 8 of four heads behind 4700 tokens, 128 of their own 44.5 -> 33.2 us, 30 35.2 -> 30.0, none
+// 27.7 -> 29.0; 4 x 32 heads behind 3400 38.9 -> 34.1, 30.7 -> 33.8, 29.6 -> 33.9; with 512 streams, 16 x 32 behind 2300, 38.7 -> 41.2 instead.
 static PrefixPlan prefix_plan(int tokens, int interval, int B, int G, int Hkv)
 {
     PrefixPlan p{};
@@ -751,7 +756,12 @@ static PrefixPlan prefix_plan(int tokens, int interval, int B, int G, int Hkv)
     p.interval = interval > 0 ? interval : tokens;
     p.n_int = int(((long long)tokens + p.interval - 1) / p.interval);
     p.n = (long long)p.n_int * Hkv * p.row_tiles;
-    const int units = Hkv * p.row_tiles, each = std::min(2 * kSMs / units, p.n_int), places = 2 * kSMs;
+    const int units = Hkv * p.row_tiles, places = 2 * kSMs - ((long long)B * Hkv <= 256 ? 32 : 0);
+    int each = std::min(places / units, p.n_int);
+    if (each) {
+        const int longest = (p.n_int + each - 1) / each;
+        each = (p.n_int + longest - 1) / longest;
+    }
     const long long even = (p.n + places - 1) / places, whole = each ? (p.n_int + each - 1) / each : even;
     p.each = whole * p.interval <= even * p.interval + 300 ? each : 0;
     p.ctas = p.each ? units * each : int(std::min((long long)places, p.n));

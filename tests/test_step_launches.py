@@ -53,7 +53,8 @@ def test_refused_beside_follows(nth):
 
 @pytest.mark.parametrize("B,Hq,Hkv,P,interval,ctas", [
     (1, 1, 1, 1, 0, 1), (1, 1, 1, 100000, 0, 1),          # no checkpoints: one run a head
-    (1, 1, 1, 8192, 128, 64), (4, 32, 32, 8192, 128, 288), (64, 32, 32, 8192, 128, 288), (129, 32, 32, 8192, 128, 256),
+    (1, 1, 1, 8192, 128, 64), (4, 32, 32, 8192, 128, 256), (4, 32, 32, 9216, 128, 256), (64, 32, 32, 8192, 128, 256), (64, 32, 32, 9216, 128, 288),
+    (129, 32, 32, 8192, 128, 256),
     (2, 150, 150, 1000, 96, PLACES), (160, 256, 32, 70, 32, PLACES), (1, 400, 400, 64, 64, PLACES), (1, 200, 200, 640, 64, 200)])
 def test_ctas_of_the_prefix(B, Hq, Hkv, P, interval, ctas):
     rc, got = prefix(B, Hq, Hkv, P, interval)
