@@ -18,7 +18,7 @@
 // So K, V and the weights are pairs, rounded number and remainder (22 bits), for three more products, and sums are fp32: what is left are
 // the fp16 queries and results that every step of the library has.  The pairs of the weights cost 1 % (64 sequences 69.4 -> 70.4 us).
 //
-// 8192 tokens of 32 heads, 4-bit: 58 us for 4 sequences, 70 us for 64, 85 us for 128; 16000 of 8 heads, 2-bit, 47 us for 32 x 4.  The bytes
+// 8192 tokens of 32 heads, 4-bit: 57 us for 4 sequences, 65 us for 64, 79 us for 128; 16000 of 8 heads, 2-bit, 45 us for 32 x 4.  The bytes
 // would take 5 us.  The scans bound it: 256 recurrences of some 20 instructions a token and head, 10.2 cycles a value and scheduler in a
 // bare loop, here a third more for waits among the warps, and a sixth of the time is filling and emptying (first words 2 us, results 3 us).
 // Tiles of 64 tokens, worked on in halves: within 3 % of that, but 15.2 instead of 14.0 us where the prefix has 300 tokens.

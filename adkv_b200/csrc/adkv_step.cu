@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
 // The token is the lowest index of the largest result (a NaN counts as larger than anything), -1 where all are -inf.
 //
 // One row is bound by latency (5.2 us for 32000 tokens: launch, history, cluster barrier).  64 rows of 128256 bf16 logits with bias, mask and
-// 4000 tokens of history take 20.2 us, their bytes 5.4: 3 us until the history is counted, 5.5 for the penalties, which nearly every warp
+// 4000 tokens of history take 20.0 us, their bytes 5.4: 3 us until the history is counted, 5.5 for the penalties, which nearly every warp
 // has to do for some lane, and 9 for the rest, which is as much issue as it is 84 MB through L2 (a bias is four bytes a token and row).
 // A cluster of up to eight CTAs shares a row; each counts the history's tokens
 // that fall into its part in shared memory (integer additions, so the order does not matter) and then passes over its part once, 16
@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) process_logits_kernel(const 
     const float rep = a.repetition ? a.repetition[b] : a.repetition1, pres = a.presence ? a.presence[b] : a.presence1,
                 freq = a.frequency ? a.frequency[b] : a.frequency1;
     const int *history = a.history ? a.history + b * a.stride_history : nullptr;
+    const int first_id = history && int(threadIdx.x) < a.history_cap ? history[threadIdx.x] : -1;
     const int n_history = !history ? 0 : a.history_lens ? min(max(a.history_lens[b], 0), a.history_cap) : a.history_cap;
 
     const auto whole = [&](int p) { return p * N >= skew && p * N - skew + N <= a.V; };   // all of a pack lies in the row
@@ -504,12 +505,13 @@ __global__ void __launch_bounds__(kLogitThreads, 2) process_logits_kernel(const 
             }
         };
         fetch(p0 + threadIdx.x);
-        if (n_history) {
+        if (history) {   // cleared before the length is known, which is on its way with the first ids
+            int id = first_id;
             for (int i = threadIdx.x; i < ((p1 - p0) * N / PER + 3) / 4; i += kLogitThreads) reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
 #pragma unroll 8
             for (int i = threadIdx.x; i < n_history; i += kLogitThreads) {
-                const int id = history[i];
+                if (i >= kLogitThreads) id = history[i];
                 const uint32_t e = uint32_t(id) + uint32_t(skew), group = e / (32 * N);
                 const int l = int(group >> log_ranks << 5 | (e / N & 31)) - p0;   // the CTA's pack that holds it, if it is the CTA's
                 if (id >= 0 && id < a.V && (group & (ranks - 1)) == rank && l >= 0 && l < p1 - p0) {
