@@ -57,13 +57,15 @@ struct Four<float> {
 // in fp32, one rounding at the end; products and sums of the rotation are rounded one by one, as the torch expression in e2e_llama
 // does.  Values pass through, so that all of [B, T, (Hq + 2 Hkv) D] leaves in the [B, H, T, D] layout that the caches take.
 //
-// Every element is read and written once, the tables are 1 % of it: 8191 tokens of 48 heads of 128 take 44.5 us, 0.70 of the rate of a copy,
-// 16 x 777 tokens of 48 heads of 256 121 us, 0.77; the issue slots are 73 % busy.  128 single tokens take 3.2 us, a launch and a round
-// trip.  A lane holds eight channels of a head, four pairs, so that both halves of a pair are its own and nothing but the sum of squares
-// crosses lanes; D / 8 lanes share a head, and a thread takes the same channels of up to kRopeRows heads of one token, so cosines and
-// sines are loaded once for them.  A CTA goes on from token to token, and the next two are on their way to shared memory while it works
-// on one: with a token a CTA, half of the time nothing is.  Every thread reads what it has copied itself, so nothing has to be waited for
-// but its own copies.
+// Every element is read and written once, the tables are 1 % of it: 8191 tokens of 48 heads of 128 take 39.6 us, 0.79 of the rate of a copy,
+// 16 x 777 tokens of 48 heads of 256 102.8 us, 0.91.  128 single tokens take 2.9 us, a launch and a round trip.  A lane holds eight or
+// sixteen channels of a head, in pairs of groups of four, so that both halves of a pair are its own and nothing but the sum of squares
+// crosses lanes; a thread takes the same channels of up to kRopeRows heads of one token, so cosines and sines are loaded once for them.
+// A CTA goes on from token to token, and the next two are on their way to shared memory while it works on one: with a token a CTA, half
+// of the time nothing is.  Every thread reads what it has copied itself, so nothing has to be waited for but its own copies, and CTAs are
+// as small as they may be for the registers to hold many tokens: 256 threads and eight channels a lane 44.0 and 120 us, and with sixteen 43.6
+// and 115, 128 threads 45.9 and 102; of 64 threads with one head each 44.2 and 119, with three 45.8 and 120, 32 threads 40.5 and 103, four
+// tokens on their way 45.7 and 117.
 struct RopeArgs {
     const void *qkv;
     long long stride_b, stride_t;      // elements
@@ -76,19 +78,22 @@ struct RopeArgs {
     int rows;                          // heads of a thread, at most kRopeRows
     float eps;
 };
-constexpr int kRopeThreads = 256, kRopeRows = 4;
+constexpr int kRopeThreads = 64, kRopeRows = 2;
+constexpr int kRopeCtas = 12;            // of an SM
+template <int D>
+__host__ __device__ constexpr int rope_units() { return D >= 128 ? 2 : 1; }   // groups of eight channels of a lane
 
 template <int D, class In>
-__host__ __device__ constexpr int rope_slot_bytes() { return kRopeRows * (D == 512 ? 2 : 1) * 2 * kRopeThreads * int(sizeof(typename Four<In>::Raw)); }   // of a stage
+__host__ __device__ constexpr int rope_slot_bytes() { return kRopeRows * rope_units<D>() * 2 * kRopeThreads * int(sizeof(typename Four<In>::Raw)); }   // of a stage
 template <int D, class In>
-__host__ __device__ constexpr int rope_stages() { return rope_slot_bytes<D, In>() > 32768 ? 2 : 3; }
+__host__ __device__ constexpr int rope_stages() { return rope_slot_bytes<D, In>() > 4096 ? 2 : 3; }   // so that all CTAs find room
 __device__ __forceinline__ void copy_async(uint2 *dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory"); }
 __device__ __forceinline__ void copy_async(float4 *dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory"); }
 
 template <int D, class In, class Out>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ RopeArgs a)
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas) norm_rope_kernel(const __grid_constant__ RopeArgs a)
 {
-    constexpr int UNITS = D == 512 ? 2 : 1, LANES = D / 8 / UNITS;   // lanes of a head, and groups of eight channels of a lane
+    constexpr int UNITS = rope_units<D>(), LANES = D / 8 / UNITS;   // LANES: of a head
     constexpr int HEADS = kRopeThreads / LANES;                      // heads that the CTA takes side by side
     using Raw = typename Four<In>::Raw;
     const int lane = threadIdx.x % LANES, H = a.Hq + 2 * a.Hkv, half = a.rot / 2;
@@ -572,32 +577,28 @@ using namespace adkv;
 
 ADKV_DEFINE_TU_STATUS(adkv_tu_status_step)
 
-// CTAs that the chip holds of the kernel, four an SM.
-constexpr long long kRopePlaces = 4 * kSMs;
-
 template <int D, class In, class Out>
-static int launch_rope_kernel(const RopeArgs &a, dim3 grid, cudaStream_t s)
+static int launch_rope_kernel(RopeArgs a, cudaStream_t s)
 {
-    constexpr int bytes = rope_stages<D, In>() * rope_slot_bytes<D, In>();
-    const auto kernel = norm_rope_kernel<D, In, Out>;
-    if (bytes > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return launch_status();
-    kernel<<<grid, kRopeThreads, bytes, s>>>(a);
+    constexpr int bytes = rope_stages<D, In>() * rope_slot_bytes<D, In>(), heads = kRopeThreads / (D / 8 / rope_units<D>());
+    static_assert(bytes <= 48 * 1024, "");
+    constexpr long long places = kSMs * std::min(kRopeCtas, 227 * 1024 / (bytes + 1024));   // CTAs that the chip holds
+    const int each = (a.Hq + 2 * a.Hkv + heads - 1) / heads, groups = (each + kRopeRows - 1) / kRopeRows;
+    a.rows = (each + groups - 1) / groups;
+    const dim3 grid(std::min((long long)a.tokens, std::max(1ll, places / groups)), groups);
+    norm_rope_kernel<D, In, Out><<<grid, kRopeThreads, bytes, s>>>(a);
     return launch_status();
 }
 
 template <int D>
-static int launch_rope(RopeArgs a, int in_type, int out_type, cudaStream_t s)
+static int launch_rope(const RopeArgs &a, int in_type, int out_type, cudaStream_t s)
 {
-    constexpr int heads = kRopeThreads / (D / 8 / (D == 512 ? 2 : 1));
-    const int each = (a.Hq + 2 * a.Hkv + heads - 1) / heads, groups = (each + kRopeRows - 1) / kRopeRows;
-    a.rows = (each + groups - 1) / groups;
-    const dim3 grid(std::min((long long)a.tokens, std::max(1ll, kRopePlaces / groups)), groups);
     switch (in_type * 4 + out_type) {
-    case ADKV_T_F16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __half, __half>(a, grid, s);
-    case ADKV_T_BF16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __nv_bfloat16, __half>(a, grid, s);
-    case ADKV_T_BF16 * 4 + ADKV_T_BF16: return launch_rope_kernel<D, __nv_bfloat16, __nv_bfloat16>(a, grid, s);
-    case ADKV_T_F32 * 4 + ADKV_T_F16: return launch_rope_kernel<D, float, __half>(a, grid, s);
-    case ADKV_T_F32 * 4 + ADKV_T_F32: return launch_rope_kernel<D, float, float>(a, grid, s);
+    case ADKV_T_F16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __half, __half>(a, s);
+    case ADKV_T_BF16 * 4 + ADKV_T_F16: return launch_rope_kernel<D, __nv_bfloat16, __half>(a, s);
+    case ADKV_T_BF16 * 4 + ADKV_T_BF16: return launch_rope_kernel<D, __nv_bfloat16, __nv_bfloat16>(a, s);
+    case ADKV_T_F32 * 4 + ADKV_T_F16: return launch_rope_kernel<D, float, __half>(a, s);
+    case ADKV_T_F32 * 4 + ADKV_T_F32: return launch_rope_kernel<D, float, float>(a, s);
     default: return ADKV_E_TYPE;
     }
 }
