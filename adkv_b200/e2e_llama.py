@@ -202,10 +202,12 @@ class ADKVLlama:
                                   q_weight=L.get("q_norm"), k_weight=L.get("k_norm"), eps=self.s.norm_eps)
 
     def _remember(self, tokens: torch.Tensor) -> None:
-        """Add one token per sequence to the history that ``logit_rules`` look at."""
+        """Add one token per sequence to the history that ``logit_rules`` look at.  How many there are is on the device: replayed steps
+        behind the last place, which have no results either, write that place again."""
         if self.logit_rules is not None:
-            self.history.scatter_(1, self.history_lens.long()[:, None], tokens.int()[:, None])
-            self.history_lens += 1
+            at = self.history_lens.clamp(max=self.history.shape[1] - 1)
+            self.history.scatter_(1, at.long()[:, None], tokens.int()[:, None])
+            self.history_lens.copy_(at + 1)
 
     def _choose(self, logits: torch.Tensor) -> torch.Tensor:
         if self.logit_rules is None:
@@ -345,13 +347,13 @@ class ADKVLlama:
         """One decode step in which nothing on the host depends on the position: the token count lives in
         ``self.seq_lens`` on the device (read by the attention kernel and the RoPE lookup, incremented at the
         end), so the recorded sequence of launches is the same for every step."""
-        self._remember(ids)
         positions = self.seq_lens + self.n_shared if self.n_shared else self.seq_lens
         x = self.embed[ids][:, None, :]
         for L in self.layers:
             x = x + self._allreduce(self._attn_partial(L, x, None, seq_lens=self.seq_lens, positions=positions))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.seq_lens += 1
+        self._remember(ids)
         return self._head(x)
 
     @torch.no_grad()
@@ -391,12 +393,12 @@ class ADKVLlama:
     def decode(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B] (the tokens at position T) -> next-token ids [B]; appends position T to the caches."""
         T = self.T
-        self._remember(ids)
         x = self.embed[ids][:, None, :]                                                  # [B, 1, dm]
         for L in self.layers:
             x = x + self._allreduce(self._attn_partial(L, x, T))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.T = T + 1
+        self._remember(ids)              # once nothing can refuse the step any more
         return self._head(x)
 
 
