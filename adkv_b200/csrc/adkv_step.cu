@@ -158,12 +158,14 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) norm_rope_kernel(cons
         int pos = a.start + p.t;
         if (a.positions) pos = a.per_token ? a.positions[p.b * a.T + p.t] : int(uint32_t(a.positions[p.b]) + uint32_t(p.t));   // behind the largest int: negative
         float c[UNITS][4], s[UNITS][4];
+        bool turns[UNITS];   // channels behind the rotated ones are copied (0 times an infinite neighbour is not 0); without a position all are NaN
         const bool inside = pos >= 0 && pos < a.table_rows;
         if (!inside && threadIdx.x == 0 && blockIdx.y == 0) atomicExch(&g_status, kStatPosition);
         const float *cos = a.cos + (long long)pos * a.table_stride, *sin = a.sin + (long long)pos * a.table_stride;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const int pair = 4 * (lane + LANES * u);
+            turns[u] = pair < half || !inside;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 c[u][i] = inside ? 1.f : __int_as_float(0x7fc00000);
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) norm_rope_kernel(cons
                     first = __fsub_rn(__fmul_rn(was, co), __fmul_rn(second, si));
                     second = __fadd_rn(__fmul_rn(second, co), __fmul_rn(was, si));
                 };
-                if (!is_v) {
+                if (!is_v && turns[u]) {
                     if (a.interleaved) {
                         turn(p[0], p[1], c[u][0], s[u][0]); turn(p[2], p[3], c[u][1], s[u][1]);
                         turn(n[0], n[1], c[u][2], s[u][2]); turn(n[2], n[3], c[u][3], s[u][3]);
