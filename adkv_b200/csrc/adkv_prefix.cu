@@ -12,11 +12,14 @@
 //
 // Values are fp16 numbers for the products, as differences from the zero point at the start of the run: that point's share of a logit is
 // the same for the whole run and is added in fp32 to the maximum, its share of the result to the sums, so a channel far from zero keeps the
-// bits of its deviations.  They are held in units of 16, a power of two, so that differences up to a million are in range.  One fp16 number
+// bits of its deviations.  They are held in units of 16, a power of two, so that differences up to a million (16 x 65504) are in range.  One fp16 number
 // is 2^-11 of a value: with channels that reach 50, as the outliers of this library's benchmark do, logits would be off by some 1e-3 and
 // results by up to 2.7 times what its results may be off (2e-3 and 2e-3 of the value); with weights of 11 bits it would be up to 1.2 times.
 // So K, V and the weights are pairs, rounded number and remainder (22 bits), for three more products, and sums are fp32: what is left are
 // the fp16 queries and results that every step of the library has.  The pairs of the weights cost 1 % (64 sequences 69.4 -> 70.4 us).
+// fp16 numbers have no step below 2^-24: a value is off by up to 2^-21 (half of that, in units of 16) however small it is.  The denominator adds up
+// the weights as they were, so what small ones lose does not cancel; the largest therefore starts at 2^7 and grows to 2^15, which leaves a
+// loss of 2^-32 of the largest at most per token.
 //
 // 8192 tokens of 32 heads, 4-bit: 57 us for 4 sequences, 65 us for 64, 79 us for 128; 16000 of 8 heads, 2-bit, 45 us for 32 x 4.  The bytes
 // would take 5 us.  The scans bound it: 256 recurrences of some 20 instructions a token and head, 10.2 cycles a value and scheduler in a
@@ -36,7 +39,7 @@ constexpr int kPreWords = 4, kPreKV = 3, kPreP = 2;   // tiles of words, of K an
 constexpr int kPreWarps = 14;                 // 0-3: K, 4-7: V (a channel a thread), 8-11: softmax (a row a thread), 12, 13: products
 constexpr int kPreThreads = 32 * kPreWarps;
 constexpr float kPreUnit = 16.f;              // values are held in units of this
-constexpr float kPreSlack = 8.f;              // a row's sums are rescaled when its maximum has grown by 2^this: weights stay below 2^8
+constexpr float kPreTop = 7.f, kPreSlack = 8.f;   // the weight of a row's maximum is 2^kPreTop; sums are rescaled when it has grown by 2^kPreSlack
 
 struct PrefixArgs {
     const __half *q;                 // [B, Hq, kD]
@@ -144,7 +147,7 @@ __device__ __forceinline__ void prefix_window(uint32_t w, const FieldConsts<BITS
                                                                            pack_remainder(hi.z, x[4], x[5]), pack_remainder(hi.w, x[6], x[7]));
 }
 
-__device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreSlack
+__device__ __forceinline__ float exp2_fast(float v)   // underflows to zero; the arguments are at most kPreTop + kPreSlack
 {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -371,9 +374,9 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < kPreTok; j += 2) top = fmaxf(fmaxf(top, __uint_as_float(v[j])), __uint_as_float(v[j + 1]));
                 top *= f;
-                const bool grown = top > m + kPreSlack;   // the first tile: m is -inf
+                const bool grown = top > m + (kPreTop + kPreSlack);   // the first tile: m is -inf
                 if (__any_sync(kFull, grown)) {
-                    const float corr = grown ? exp2_fast(m - top) : 1.f;
+                    const float corr = grown ? exp2_fast(m - (top - kPreTop)) : 1.f;
                     if (i > 0) {
                         // all sums so far are in: O can be changed
                         if (!(ok = mbar_wait(&sh.odone[(tile - 1) % kPreKV], (tile - 1) / kPreKV & 1, kStatVWait))) break;
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) prefix_kernel(const __grid_con
                         }
                     }
                     l *= corr;
-                    if (grown) m = top;
+                    if (grown) m = top - kPreTop;
                 }
                 float sum[4] = {};
 #pragma unroll

@@ -303,7 +303,8 @@ long long adkv_decode_attn_prefix_scratch_bytes(int B, int Hq, int Hkv, int pref
 /* Decode step of B sequences behind one prefix: query b attends to the prefix, to the tokens that sequence b has cached itself and to
  * its new token, which is appended.  Same result as adkv_decode_attn_varlen with tail states and ADKV_FLAG_FAST_REPLAY on caches that
  * hold prefix and own tokens in one piece, up to summation order and the rounding of the prefix's dequantised values and weights to
- * pairs of fp16 numbers (22 bits; values as differences from the zero points at the start of a run of intervals, in range up to 2^19).
+ * pairs of fp16 numbers: 2^-22 of a value, but not less than 2^-21 (values as differences from the zero points at the start of a run of
+ * intervals, in range up to a million), and 2^-22 of a weight, but not less than 2^-32 of the row's largest.
  *   k_cache, v_cache  uint32 [B, Hkv, n_super_cap, D]: the sequences' own tokens, from index 0 on.  The recurrence enters them with the
  *          state behind the prefix (prefix->k_tail, v_tail); fill them with ADKV_FLAG_TAIL_START, or with adkv_append_kv from T = 0 on.
  *   k_tail, v_tail    float [B, Hkv, 2, D], required, in/out: the state behind the last own token, the prefix's where there is none.
