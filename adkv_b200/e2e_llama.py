@@ -80,7 +80,8 @@ class ADKVLlama:
         """``shared_tokens``: room for a prompt that all sequences share (:meth:`prefill_shared`; fused, fp32 arithmetic, head dim 128, no
         ``ckpt_interval``), kept once and with state checkpoints every ``shared_interval`` tokens; ``max_tokens`` are then each sequence's
         own.  ``logit_rules``: arguments of :func:`step.process_logits` for the choice of every next token (``repetition``, ``presence``,
-        ``frequency``, ``bias``, ``mask``); the history they look at is the tokens a sequence was given and has generated.
+        ``frequency``, ``bias``, ``mask``); the history they look at is the tokens a sequence was given and has generated.  A sequence
+        that they leave no token has ended: its token is -1 then and in every later step, which only takes it along with the others.
 
         ``fast``: None = contracted replay wherever tail states keep the stored codes exact (the fused step in the
         fp32 arithmetic), canonical replay otherwise.  ``peers``: the other tensor-parallel shards when all of them
@@ -209,10 +210,15 @@ class ADKVLlama:
             self.history.scatter_(1, at.long()[:, None], tokens.int()[:, None])
             self.history_lens.copy_(at + 1)
 
-    def _choose(self, logits: torch.Tensor) -> torch.Tensor:
+    def _embed(self, ids: torch.Tensor) -> torch.Tensor:
+        return self.embed[ids if self.logit_rules is None else ids.clamp(min=0)]      # sequences that have ended: token 0
+
+    def _choose(self, logits: torch.Tensor, ids: torch.Tensor | None = None) -> torch.Tensor:
+        """The next tokens; ``ids``: those before them, of which the -1 stay."""
         if self.logit_rules is None:
             return logits.argmax(-1)
-        return step.process_logits(logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[1].long()
+        tok = step.process_logits(logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[1].long()
+        return tok if ids is None else torch.where(ids < 0, ids, tok)
 
     def _ck(self, L):
         return dict(k_ckpt=L["kck"], v_ckpt=L["vck"], ckpt_interval=self.ckpt_interval) if self.ckpt_interval else {}
@@ -312,10 +318,10 @@ class ADKVLlama:
         self._mark("norm_mlp")
         return out
 
-    def _head(self, x):
+    def _head(self, x, ids=None):
         last = _rms_norm(x[:, 0], self.final_norm, self.s.norm_eps)
         self.last_logits = last @ self.lm_head.T
-        tok = self._choose(self.last_logits)
+        tok = self._choose(self.last_logits, ids)
         self._mark("final_norm_lm_head")
         return tok
 
@@ -348,13 +354,13 @@ class ADKVLlama:
         ``self.seq_lens`` on the device (read by the attention kernel and the RoPE lookup, incremented at the
         end), so the recorded sequence of launches is the same for every step."""
         positions = self.seq_lens + self.n_shared if self.n_shared else self.seq_lens
-        x = self.embed[ids][:, None, :]
+        x = self._embed(ids)[:, None, :]
         for L in self.layers:
             x = x + self._allreduce(self._attn_partial(L, x, None, seq_lens=self.seq_lens, positions=positions))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.seq_lens += 1
         self._remember(ids)
-        return self._head(x)
+        return self._head(x, ids)
 
     @torch.no_grad()
     def capture_decode(self, warmup_ids: torch.Tensor, warmup_steps: int = 3) -> torch.Tensor:
@@ -393,13 +399,13 @@ class ADKVLlama:
     def decode(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B] (the tokens at position T) -> next-token ids [B]; appends position T to the caches."""
         T = self.T
-        x = self.embed[ids][:, None, :]                                                  # [B, 1, dm]
+        x = self._embed(ids)[:, None, :]                                                 # [B, 1, dm]
         for L in self.layers:
             x = x + self._allreduce(self._attn_partial(L, x, T))
             x = x + self._allreduce(self._mlp_partial(L, x))
         self.T = T + 1
         self._remember(ids)              # once nothing can refuse the step any more
-        return self._head(x)
+        return self._head(x, ids)
 
 
 @torch.no_grad()
@@ -408,13 +414,13 @@ def step_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
     :meth:`ADKVLlama.decode`, with each all-reduce replaced by the sum of the shards' partial results.  Used to
     test the sharding (head slices of weights and ADKV parameters, caches per shard) without several GPUs."""
     T = shards[0].T
-    x = shards[0].embed[ids][:, None, :]
+    x = shards[0]._embed(ids)[:, None, :]
     for li in range(len(shards[0].layers)):
         x = x + torch.stack([m._attn_partial(m.layers[li], x, T) for m in shards]).sum(0)
         x = x + torch.stack([m._mlp_partial(m.layers[li], x) for m in shards]).sum(0)
     for m in shards:
         m.T = T + 1
-    tok = shards[0]._head(x)
+    tok = shards[0]._head(x, ids)
     for m in shards[1:]:
         m.last_logits = shards[0].last_logits
     return tok

@@ -58,3 +58,40 @@ def test_a_refused_step_leaves_the_history_alone(monkeypatch):
         with pytest.raises(RuntimeError, match="CUDA tensor"):       # the attention has no CPU path
             m.decode(tokens(1, B))
     assert m.history_lens.tolist() == [0] * B and torch.equal(m.history, before) and m.T == 4
+
+
+def allow(*rows):
+    """Mask words [B, ceil(V / 32)]: the tokens that each row allows."""
+    m = torch.zeros(B, (BARE.vocab + 31) // 32, dtype=torch.int64)
+    for b, row in enumerate(rows):
+        for t in row:
+            m[b, t // 32] |= 1 << (t % 32)
+    return torch.where(m >= 1 << 31, m - (1 << 32), m).int()
+
+
+def test_a_sequence_that_is_left_no_token_has_ended(monkeypatch):
+    """Its token is -1 from then on, whatever the rules allow later; no row of the embedding stands for it, and the others go on."""
+    mask = allow(range(50), range(50), [7, 40])
+    m, other = (model(monkeypatch, 12, mask=x, frequency=0.5) for x in (mask, allow(range(50), range(50), [7, 40])))
+    ids = tokens(2, B, 4)
+    tok = m.prefill(ids)
+    assert torch.equal(tok, other.prefill(ids)) and int(tok[2]) in (7, 40)
+    mask[1] = 0
+    for i in range(5):
+        before = tok
+        tok, want = m.decode(tok), other.decode(tok.clamp(min=0))
+        assert torch.equal(m.last_logits, other.last_logits)              # taken along with token 0
+        assert tok.tolist() == [int(want[0]), -1, int(want[2])]
+        assert m.history[:, 4 + i].tolist() == before.tolist()
+        if i == 2:
+            mask[1] = -1
+    assert m.history_lens.tolist() == [9] * B
+    mask[0] = 0
+    fresh = model(monkeypatch, 12, mask=mask)
+    assert int(fresh.prefill(ids)[0]) == -1
+
+
+def test_without_rules_tokens_are_taken_as_they_are(monkeypatch):
+    m = ADKVLlama(BARE, B, 8, device="cpu")
+    tok = m.prefill(tokens(3, B, 2))
+    assert torch.equal(tok, m.last_logits.argmax(-1)) and torch.equal(m.decode(tok), m.last_logits.argmax(-1))
