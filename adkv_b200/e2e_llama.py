@@ -70,6 +70,14 @@ def _apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.
     return (xf * cos + rot * sin).to(x.dtype)
 
 
+def _in_turn(logits: torch.Tensor) -> torch.Tensor:
+    """logits [B, V] -> tokens [B]: of row b the b-th largest above -inf, counted round where there are fewer; -1 where there is none."""
+    top, at = logits.float().topk(min(logits.shape), -1)
+    n = (top != float("-inf")).sum(-1)
+    b = torch.arange(logits.shape[0], device=logits.device) % n.clamp(min=1)
+    return torch.where(n > 0, at.gather(-1, b[:, None])[:, 0], -1)
+
+
 class ADKVLlama:
     """One tensor-parallel shard of the model with its packed KV caches."""
 
@@ -255,7 +263,7 @@ class ADKVLlama:
     @torch.no_grad()
     def prefill_shared(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [P]: the prompt that all sequences share, prefilled once -> their first tokens [B], the most likely ones in turn (the same
-        for all would be the same completion)."""
+        for all would be the same completion): sequence b takes the b-th that its rules allow, counted round where those are fewer."""
         P = ids.numel()
         assert ids.dim() == 1 and 0 < P <= self.shared_tokens and self.T == 0 and self.shared is None
         x = self.embed[ids][None]
@@ -279,9 +287,8 @@ class ADKVLlama:
         if self.logit_rules is not None:
             self.history[:, :P] = ids
             self.history_lens.fill_(P)
-            logits = step.process_logits(self.last_logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[0]
-            return logits.float().topk(self.B, -1).indices.diagonal()
-        return self.last_logits[0].float().topk(self.B).indices
+            return _in_turn(step.process_logits(self.last_logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[0])
+        return _in_turn(self.last_logits)
 
     # ------------------------------------------------------------------ the two halves of a layer, before the all-reduce
     def _attn_partial(self, L, x, T, seq_lens=None, positions=None):

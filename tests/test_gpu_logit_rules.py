@@ -60,3 +60,24 @@ def test_replayed_steps_behind_the_last_place():
         tok = m.decode_replay(tok)
     assert m.history_lens.tolist() == [P + room + 1] * B and torch.equal(m.history[:, :P + room], before)
     assert bool(((tok >= -1) & (tok < TINY.vocab)).all()) and gemv.device_status() in (6, 8)
+
+
+@pytest.mark.parametrize("B", [2, 6])
+def test_first_tokens_behind_a_shared_prompt_are_allowed(B):
+    mask = _mask(B, 0)
+    mask[:, 1] = 0b1110                  # tokens 33, 34, 35
+    mask[B - 1] = 0                      # none
+    m = ADKVLlama(TINY, B, 8, device="cuda", seed=3, shared_tokens=40, logit_rules=dict(mask=mask))
+    tok = m.prefill_shared(_ids(5, 33))
+    order = (33 + m.last_logits[0, 33:36].float().argsort(descending=True)).tolist()
+    assert tok.tolist() == [order[b % 3] for b in range(B - 1)] + [-1]
+    nxt = m.decode(tok)
+    assert all(33 <= t <= 35 for t in nxt.tolist()[:-1]) and int(nxt[-1]) == -1 and gemv.device_status() == 0
+
+
+def test_more_sequences_behind_a_shared_prompt_than_tokens():
+    shape = LlamaShape(**{**TINY.__dict__, "vocab": 5})
+    m = ADKVLlama(shape, 8, 4, device="cuda", seed=3, shared_tokens=16)
+    tok = m.prefill_shared(_ids(5, 9) % 5)
+    order = m.last_logits[0].float().argsort(descending=True).tolist()
+    assert tok.tolist() == [order[b % 5] for b in range(8)] and m.decode(tok).shape == (8,)

@@ -95,3 +95,20 @@ def test_without_rules_tokens_are_taken_as_they_are(monkeypatch):
     m = ADKVLlama(BARE, B, 8, device="cpu")
     tok = m.prefill(tokens(3, B, 2))
     assert torch.equal(tok, m.last_logits.argmax(-1)) and torch.equal(m.decode(tok), m.last_logits.argmax(-1))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (5, 5), (4, 50), (7, 3), (9, 1)])
+def test_first_tokens_in_turn(rows, vocab):
+    """Row b's b-th most likely token, round and round where the vocabulary or what the row allows is smaller than the batch."""
+    g = torch.Generator().manual_seed(rows * vocab)
+    logits = torch.randn(rows, vocab, generator=g).half()
+    allowed = torch.rand(rows, vocab, generator=g) < torch.linspace(0, 1, rows)[:, None]
+    for x in (logits, logits[:1].expand(rows, vocab), logits.masked_fill(~allowed, -math.inf)):
+        got = e2e_llama._in_turn(x)
+        assert got.shape == (rows,) and got.dtype == torch.int64
+        for b in range(rows):
+            order = sorted((v for v in range(vocab) if x[b, v] > -math.inf), key=lambda v: -float(x[b, v]))
+            if not order:
+                assert int(got[b]) == -1
+            else:
+                assert x[b, int(got[b])] == x[b, order[b % len(order)]]      # of equal logits either
