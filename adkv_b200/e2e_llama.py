@@ -210,6 +210,12 @@ class ADKVLlama:
         return step.norm_rope_qkv(h @ L["wqkv"].T, self.hq, self.hkv, self.cos[:, :half], self.sin[:, :half], start=start, positions=positions,
                                   q_weight=L.get("q_norm"), k_weight=L.get("k_norm"), eps=self.s.norm_eps)
 
+    def _remember_prompt(self, ids: torch.Tensor) -> None:
+        """Begin the history with a prompt [B, P] or [P]."""
+        if self.logit_rules is not None:
+            self.history[:, :ids.shape[-1]] = ids
+            self.history_lens.fill_(ids.shape[-1])
+
     def _remember(self, tokens: torch.Tensor) -> None:
         """Add one token per sequence to the history that ``logit_rules`` look at.  How many there are is on the device: replayed steps
         behind the last place, which have no results either, write that place again."""
@@ -255,9 +261,7 @@ class ADKVLlama:
             logits.append(last @ self.lm_head.T)
         self.T = Tp
         self.last_logits = torch.cat(logits)
-        if self.logit_rules is not None:
-            self.history[:, :Tp] = ids
-            self.history_lens.fill_(Tp)
+        self._remember_prompt(ids)
         return self._choose(self.last_logits)
 
     @torch.no_grad()
@@ -284,9 +288,8 @@ class ADKVLlama:
             L["shared"] = prefix
         self.shared_scratch = torch.empty(gemv.prefix_scratch_bytes(self.B, self.hq, prefixes[0]), dtype=torch.uint8, device=self.dev)
         self.last_logits = (_rms_norm(x[:, -1], self.final_norm, self.s.norm_eps) @ self.lm_head.T).expand(self.B, -1)
+        self._remember_prompt(ids)
         if self.logit_rules is not None:
-            self.history[:, :P] = ids
-            self.history_lens.fill_(P)
             return _in_turn(step.process_logits(self.last_logits, history=self.history, history_lens=self.history_lens, **self.logit_rules)[0])
         return _in_turn(self.last_logits)
 
@@ -427,6 +430,7 @@ def step_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
         x = x + torch.stack([m._mlp_partial(m.layers[li], x) for m in shards]).sum(0)
     for m in shards:
         m.T = T + 1
+        m._remember(ids)
     tok = shards[0]._head(x, ids)
     for m in shards[1:]:
         m.last_logits = shards[0].last_logits
@@ -451,6 +455,7 @@ def prefill_together(shards: list, ids: torch.Tensor) -> torch.Tensor:
         x = x + torch.stack([m._mlp_partial(m.layers[li], x) for m in shards]).sum(0)
     for m in shards:
         m.T = Tp
+        m._remember_prompt(ids)
     return shards[0]._head(x[:, -1:])
 
 

@@ -112,3 +112,18 @@ def test_first_tokens_in_turn(rows, vocab):
                 assert int(got[b]) == -1
             else:
                 assert x[b, int(got[b])] == x[b, order[b % len(order)]]      # of equal logits either
+
+
+def test_shards_stepped_together_keep_the_history(monkeypatch):
+    """Prefill and steps of co-resident shards look at the history that one model does; every shard holds it."""
+    one = model(monkeypatch, 12, frequency=30.0)
+    shards = [ADKVLlama(BARE, B, 12, device="cpu", rank=r, world=2, peers=[], logit_rules=dict(frequency=30.0)) for r in range(2)]
+    ids = tokens(6, B, 4)
+    tok = one.prefill(ids)
+    assert torch.equal(e2e_llama.prefill_together(shards, ids), tok)
+    for _ in range(6):
+        got = e2e_llama.step_together(shards, tok)
+        tok = one.decode(tok)
+        assert torch.equal(got, tok)
+    for m in shards:
+        assert torch.equal(m.history, one.history) and torch.equal(m.history_lens, one.history_lens)
