@@ -143,7 +143,8 @@ class KVCacheLayer:
 
     # ------------------------------------------------------------------ several sequences behind one
     def fork(self, batch: int, capacity_tokens: int | None = None) -> "KVCacheLayer":
-        """A layer of ``batch`` sequences whose first tokens are those cached here (one sequence, fused, with tail states, head dim 128).
+        """A layer of ``batch`` sequences whose first tokens are those cached here (one sequence, fused, with tail states, head dim 128,
+        not ``fast=False``: its steps replay in the contracted arithmetic).
 
         The tokens are shared, not copied: they are quantised already, and this layer's buffers are kept alive and read by every step of
         the new one.  This layer may be continued on its own, and forked again.  With ``checkpoint_interval`` the shared tokens are replayed
@@ -157,6 +158,8 @@ class KVCacheLayer:
         B, H, D, device = self._geom
         if B != 1 or D != 128 or not self._keeps_tails:
             raise ValueError("only a layer of one sequence with tail states and head dim 128 can be shared")
+        if self.fast is not None and not self.fast:
+            raise ValueError("steps behind a shared prefix replay in the contracted arithmetic: fast=False cannot be had")
         child = KVCacheLayer(bits=self.bits, fast=self.fast, capacity_tokens=capacity_tokens)
         child._prefix = gemv.SharedPrefix(self._k, self._v, self._n, k_tail=self._k_tail.clone(), v_tail=self._v_tail.clone(), bits=self.bits,
                                           k_ckpt=self._k_ckpt, v_ckpt=self._v_ckpt, ckpt_interval=self._interval)

@@ -85,7 +85,7 @@ class ADKVLlama:
                  rank: int = 0, world: int = 1, seed: int = 0, fused: bool = True, fast: bool | None = None,
                  ckpt_interval: int = 0, half_state: bool = False, peers: list | None = None,
                  split_channels: bool | None = None, shared_tokens: int = 0, shared_interval: int = 128, logit_rules: dict | None = None):
-        """``shared_tokens``: room for a prompt that all sequences share (:meth:`prefill_shared`; fused, fp32 arithmetic, head dim 128, no
+        """``shared_tokens``: room for a prompt that all sequences share (:meth:`prefill_shared`; fused, fp32 arithmetic, contracted replay, head dim 128, no
         ``ckpt_interval``), kept once and with state checkpoints every ``shared_interval`` tokens; ``max_tokens`` are then each sequence's
         own.  ``logit_rules``: arguments of :func:`step.process_logits` for the choice of every next token (``repetition``, ``presence``,
         ``frequency``, ``bias``, ``mask``); the history they look at is the tokens a sequence was given and has generated.  A sequence
@@ -107,6 +107,8 @@ class ADKVLlama:
         self.shared_tokens, self.shared, self.n_shared = shared_tokens, None, 0
         if shared_tokens and (not self.keeps_tails or ckpt_interval or shape.head_dim != 128):
             raise ValueError("a shared prompt needs the fused step with tail states, head dim 128 and no ckpt_interval")
+        if shared_tokens and not self.fast:
+            raise ValueError("steps behind a shared prompt replay in the contracted arithmetic: fast=False cannot be had")
         self.hq, self.hkv, self.ffn = shape.n_heads // world, shape.n_kv_heads // world, shape.ffn // world
         D, dm = shape.head_dim, shape.d_model
         g = torch.Generator(device=self.dev)

@@ -644,7 +644,8 @@ def prefix_scratch_bytes(B: int, Hq: int, prefix: SharedPrefix) -> int:
 def decode_attn_prefix(q, prefix: SharedPrefix, k_cache, v_cache, k_new, v_new, k_params, v_params, T, scaling: float, scale_min,
                        scale_max, *, k_tail: torch.Tensor, v_tail: torch.Tensor, tail_keep: bool = False,
                        out: torch.Tensor | None = None, scratch: torch.Tensor | None = None):
-    """Fused decode step of B sequences that share a packed prefix, which is replayed once for all of them.
+    """Fused decode step of B sequences that share a packed prefix, which is replayed once for all of them, in the contracted
+    arithmetic (``fast=True`` of :func:`decode_attn`).
 
     ``k_cache`` / ``v_cache [B, nh_kv, n_super, DIM/4, 4, 4]`` hold the sequences' own tokens from index 0 on, quantised from the state
     behind the prefix (``encode_kv_pair(..., from_tail=True)``, ``append_kv_pair``, or earlier steps); ``T`` is their number: an int, or an
