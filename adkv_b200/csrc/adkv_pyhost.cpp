@@ -11,6 +11,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -64,7 +65,15 @@ struct Device {
     }
 };
 
-// A tensor on the current device, as at::empty makes it but without its way through the dispatcher (0.5 us).
+// Something between a call and the backend wants to see every tensor that is made (a dispatch mode, a transform): the Python path's business.
+bool watched()
+{
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Functionalize,
+                                        c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode});
+    return c10::impl::tls_local_dispatch_key_set().included_.has_any(keys);
+}
+
+// A tensor on the current device, as at::empty makes it but without its way through the dispatcher (0.5 us); not while watched().
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type)
 {
     return at::detail::empty_generic(sizes, c10::GetAllocator(at::kCUDA), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
@@ -179,7 +188,7 @@ PyObject *decode(PyObject *, PyObject *const *a, Py_ssize_t n)
 // scale_max, k_tail, v_tail, flags, out, scratch) -> the output tensor, an error code of the library, or None
 PyObject *decode_prefix(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (n != 17 || !g_prefix) Py_RETURN_NONE;
+    if (n != 17 || !g_prefix || watched()) Py_RETURN_NONE;
     try {
         const at::Tensor *kc = plain(a[2]), *vc = plain(a[3]);
         if (!kc || !vc || !kc->is_cuda() || kc->dim() != 6 || kc->size(4) != 4 || kc->size(5) != 4) Py_RETURN_NONE;
@@ -273,7 +282,7 @@ int element_type(at::ScalarType t) { return t == at::kHalf ? ADKV_T_F16 : t == a
 // None
 PyObject *norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (n != 12 || !g_rope) Py_RETURN_NONE;
+    if (n != 12 || !g_rope || watched()) Py_RETURN_NONE;
     try {
         const at::Tensor *x = plain(a[0]), *cos = plain(a[3]), *sin = plain(a[4]);
         int Hq, Hkv, start;
@@ -340,7 +349,7 @@ PyObject *norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
 // logits(logits, history, history_lens, repetition, presence, frequency, bias, mask) -> (out, tokens), an error code, or None; out is new
 PyObject *logits(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (n != 8 || !g_logits) Py_RETURN_NONE;
+    if (n != 8 || !g_logits || watched()) Py_RETURN_NONE;
     try {
         const at::Tensor *x = plain(a[0]);
         if (!x || !x->is_cuda() || x->dim() != 2 || x->stride(1) != 1) Py_RETURN_NONE;
