@@ -48,6 +48,7 @@ def norm_rope_qkv(qkv, n_heads: int, n_kv_heads: int, cos, sin, *, start: int = 
     dtype = qkv.dtype if dtype is None else dtype
     _require(dtype in (qkv.dtype, torch.float16), "dtype must be the input's or float16")
     _require(cos.shape == sin.shape and cos.dim() == 2 and cos.stride() == sin.stride(), "cos and sin must be two tables of one shape and layout")
+    _require(cos.shape[0] < 1 << 31, "the tables must have fewer than 2^31 rows")
     rot = 2 * cos.shape[1]
     _require(0 < rot <= D and rot % 8 == 0, "the rotated channels must be a multiple of 8, at most the head dim")
     for t in (cos, sin):
@@ -123,6 +124,7 @@ def process_logits(logits, *, history: torch.Tensor | None = None, history_lens:
     if history is not None:
         _require(history.dtype == torch.int32 and history.device == device and history.dim() == 2 and history.shape[0] == B and
                  (history.stride(1) == 1 or history.shape[1] <= 1), "history must be int32 [B, L] on the logits' device, rows in one piece")
+        _require(history.shape[1] < 1 << 31, "a history must have fewer than 2^31 tokens a row")
     if history_lens is not None:
         _require(history_lens.dtype == torch.int32 and history_lens.device == device and history_lens.is_contiguous() and
                  history_lens.shape == (B,), "history_lens must be a contiguous int32 [B] tensor on the logits' device")
