@@ -57,8 +57,9 @@ struct Four<float> {
 // in fp32, one rounding at the end; products and sums of the rotation are rounded one by one, as the torch expression in e2e_llama
 // does.  Values pass through, so that all of [B, T, (Hq + 2 Hkv) D] leaves in the [B, H, T, D] layout that the caches take.
 //
-// Every element is read and written once, the tables are 1 % of it: 8191 tokens of 48 heads of 128 take 39.6 us, 0.79 of the rate of a copy,
-// 16 x 777 tokens of 48 heads of 256 102.8 us, 0.91.  128 single tokens take 2.9 us, a launch and a round trip.  A lane holds eight or
+// Every element is read and written once, the tables are 1 % of it: 8191 tokens of 48 heads of 128 take 39.7 us, 0.79 of the rate of a copy,
+// 16 x 777 tokens of 48 heads of 256 102.6 us, 0.91 (replayed from a graph; called one after another 41 to 45 and 109 to 115).  128 single
+// tokens take 3.0 us, a launch and a round trip.  fp32 in, 8191 x 48 x 128: 51 us to fp16, 0.90, 74 us to fp32, 0.83.  A lane holds eight or
 // sixteen channels of a head, in pairs of groups of four, so that both halves of a pair are its own and nothing but the sum of squares
 // crosses lanes; a thread takes the same channels of up to kRopeRows heads of one token, so cosines and sines are loaded once for them.
 // A CTA goes on from token to token, and the next two are on their way to shared memory while it works on one: with a token a CTA, half
